@@ -405,6 +405,80 @@ int ti_attn_prefill_keys(const float* q, const uint16_t* k_cache, const uint16_t
  * Returns the previous mode, or -1 for a mode outside 0..3 (nothing changed). */
 int ti_attn_prefill_set_kernel(int mode);
 
+/* ------------------------------------------------------------- paged cache
+ * One layer's keys and values in pages of `page` tokens: k, v [pages][kv_heads][page][head_dim].  Token j of sequence b is
+ * place j % page of page table[b * table_ld + j / page]; entries outside [0, pages) are holes: nothing is written there, and no
+ * row sees their tokens.  A page belongs to one sequence while it is written.
+ *   kv_type TI_KV_SAME: elements of `dtype`;
+ *   TI_KV_I8: int8 q, value = q * scale of the token's block of 16 and head, k_scale / v_scale [pages][kv_heads][page / 16].
+ * Rows of a batch are ragged: row i of sequence b (row row_start[b] + i of the call) is its token len[b] - n_b + i, n_b =
+ * row_start[b + 1] - row_start[b]; len counts the call's own rows.  row_start (device, [seqs + 1], from 0, not falling) NULL: one
+ * row a sequence.  Rows behind the last sequence, and rows whose token lies outside the table (or, rotated, outside the rotation
+ * table), are left as they are; keys past the table are not there.
+ * head_dim 64, 128 or 256; page 16, 32, 64, 128 or 256; heads a multiple of kv_heads; pages * kv_heads * page / 16 and table_ld *
+ * page below 2^31; k, v and every row 16-byte aligned.  No call reads or writes memory outside the pages of its table, copies to
+ * the host or keeps anything for the next; all can be captured into graphs. */
+enum ti_paged_dtype { TI_PAGED_F16 = 0, TI_PAGED_BF16 = 1 };
+enum ti_kv_type { TI_KV_SAME = 0, TI_KV_I8 = 1 };
+enum ti_rope_kind { TI_ROPE_PAIRS = 0, TI_ROPE_HALVES = 1 };
+typedef struct ti_paged_cache {
+  void* k;
+  void* v;
+  float* k_scale;              /* TI_KV_I8 */
+  float* v_scale;
+  const int32_t* table;        /* device [seqs][table_ld]                                     */
+  const int32_t* len;          /* device [seqs]                                               */
+  int32_t table_ld, pages, page, kv_heads, head_dim, seqs;
+  int32_t dtype, kv_type;
+} ti_paged_cache;
+
+/* Rows q | k | v of a projection, [rows][(heads + 2 kv_heads) * head_dim], into the cache.  The first rot_dim dimensions of every q
+ * and k head are rotated by rope_cs[position] ([rope_len][rot_dim / 2] (cos, sin), fp32; NULL: no rotation) in fp32: dimensions
+ * (2i, 2i + 1) (TI_ROPE_PAIRS) or (i, i + rot_dim / 2) (TI_ROPE_HALVES).  q goes to q [rows][heads * head_dim] of `dtype` (heads 0:
+ * rows are k | v).  Each value is rounded once.
+ * TI_KV_I8: a block's scale is the largest of: its old one, where it holds tokens from before the call; max |new value| / 127;
+ * 2^-100.  Old tokens are moved to a larger scale, q = round(q * old / new), new ones are round(value / scale).  A value that is
+ * not finite makes its block's scale NaN. */
+typedef struct ti_paged_append_args {
+  const void* x;               /* fp32 (x_f32) or `dtype`                                     */
+  void* q;
+  const int32_t* row_start;
+  const float* rope_cs;
+  int32_t rows, heads, ldx, ldq, x_f32, rope_len, rot_dim, rope_kind;   /* rot_dim: a multiple of 16 */
+} ti_paged_append_args;
+int ti_paged_append(const ti_paged_cache* c, const ti_paged_append_args* a, ti_stream_t s);
+/* The rows' tokens back as rows k, v [rows][kv_heads * head_dim] of `dtype` (pitches ldk, ldv): tokens of a sequence that leaves
+ * the device or moves to a cache of another kind.  Tokens in holes read as 0. */
+int ti_paged_read(const ti_paged_cache* c, const int32_t* row_start, int rows, void* k, int ldk, void* v, int ldv, ti_stream_t s);
+
+/* Attention of rows q [rows][heads * head_dim] of `dtype` over the cache, out the same; query head h reads kv-head h / (heads /
+ * kv_heads).  Row at token p scores key j
+ *   s = scale * (q . k_j);  softcap > 0: s = softcap * tanh(s / softcap);  slopes: s += slopes[h] * (j - p)
+ * and sees it where first[row] <= j < len, j <= p or j < prefix[sequence], and window = 0 or j > p - window.  out = sum of softmax(s)
+ * v; a row that sees no key: 0.  What a row does not see does not reach it, infinities and NaN among it.  fp32 scores, sums and
+ * weights; weights are rounded to 16 bits (TI_KV_I8: fp16) for their products with the values.
+ * ti_paged_decode: one row a sequence (rows = seqs, row_start NULL).  ti_paged_prefill: any rows.
+ * max_len: about the longest sequence (0: the table's size); it shapes the work only, as ti_attn_decode's splits do.
+ * workspace: ti_paged_workspace_bytes of the same arguments (0: none needed; the largest of those that a program will use serves
+ * all), 16-byte aligned, contents of no meaning before or after; one launch at a time (stream order). */
+typedef struct ti_paged_attn_args {
+  const void* q;
+  void* out;
+  const int32_t* row_start;
+  const float* slopes;         /* nullable, device [heads]                                    */
+  const int32_t* first;        /* nullable, device [rows]                                     */
+  const int32_t* prefix;       /* nullable, device [seqs]                                     */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t rows, heads, ldq, ldo, max_len, window;
+  float scale, softcap;
+} ti_paged_attn_args;
+size_t ti_paged_workspace_bytes(const ti_paged_cache* c, const ti_paged_attn_args* a);
+int ti_paged_decode(const ti_paged_cache* c, const ti_paged_attn_args* a, ti_stream_t s);
+int ti_paged_prefill(const ti_paged_cache* c, const ti_paged_attn_args* a, ti_stream_t s);
+/* sizeof(ti_paged_cache), ti_paged_append_args, ti_paged_attn_args (which = 0, 1, 2): a binding checks its mirrors against them. */
+int ti_paged_struct_bytes(int which);
+
 /* The kernel ti_gemm_wq_a16 launches for plain (not group-32) weights of this shape, e.g.
  * "gemv_wq_kernel<4,4>", "gemm_rows_kernel", "gemm_wide_kernel" (bench / profile labels). */
 int ti_gemm_kernel_name(int bits, int x_kind, int M, int N, int K, char* buf, int len);

@@ -79,6 +79,30 @@ ACT_NONE, ACT_GELU_TANH, ACT_GELU_ERF = range(3)
 NORM_LAYER, NORM_RMS = 0, 1
 
 
+PAGED_F16, PAGED_BF16 = 0, 1        # ti_paged_dtype (include/ti_hip.h)
+KV_SAME, KV_I8 = 0, 1               # ti_kv_type
+ROPE_PAIRS, ROPE_HALVES = 0, 1      # ti_rope_kind
+
+
+class PagedCache(C.Structure):
+    """ti_paged_cache (include/ti_hip.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "table", "len")] + \
+        [(n, C.c_int32) for n in ("table_ld", "pages", "page", "kv_heads", "head_dim", "seqs", "dtype", "kv_type")]
+
+
+class PagedAppendArgs(C.Structure):
+    """ti_paged_append_args (include/ti_hip.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("x", "q", "row_start", "rope_cs")] + \
+        [(n, C.c_int32) for n in ("rows", "heads", "ldx", "ldq", "x_f32", "rope_len", "rot_dim", "rope_kind")]
+
+
+class PagedAttnArgs(C.Structure):
+    """ti_paged_attn_args (include/ti_hip.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "out", "row_start", "slopes", "first", "prefix", "workspace")] + \
+        [("workspace_bytes", C.c_int64)] + \
+        [(n, C.c_int32) for n in ("rows", "heads", "ldq", "ldo", "max_len", "window")] + [("scale", C.c_float), ("softcap", C.c_float)]
+
+
 class StackLayer(C.Structure):
     """ti_stack_layer (include/ti_engine.h)."""
     _fields_ = [(n, C.c_int32) for n in ("mixer", "heads", "dim", "rot_dim", "vdim", "q_rank", "kv_rank", "rot_dims")] + \
@@ -150,6 +174,7 @@ EXPORTED = [
     "ti_gqa_prep", "ti_gqa_block_elems", "ti_gqa_decode", "ti_gqa_prefill", "ti_gqa_splits", "ti_recurrent_prepare", "ti_conv",
     "ti_ssd_step", "ti_ssd_scan", "ti_ssd_norm", "ti_lru_scan", "ti_lru_step", "ti_lru_step_max_block", "ti_stack_kpad", "ti_stack_weight_bytes", "ti_stack_pack",
     "ti_stack_convert", "ti_stack_fill", "ti_dense", "ti_dense_tile", "ti_dense_args_bytes", "ti_rownorm", "ti_rownorm_routes", "ti_route", "ti_route_max_tiles",
+    "ti_paged_append", "ti_paged_read", "ti_paged_workspace_bytes", "ti_paged_decode", "ti_paged_prefill", "ti_paged_struct_bytes",
     "ti_latent_prep", "ti_latent_prepare", "ti_latent_attn_decode", "ti_latent_attn_splits", "ti_latent_attn_prefill", "ti_latent_attn_out",
 ]
 
@@ -215,6 +240,13 @@ def lib() -> C.CDLL:
         L.ti_attn_prefill.argtypes = [vp, vp, vp, i32, vp, i32, i32, i32, i32, vp, vp]
         L.ti_attn_prefill_keys.argtypes = [vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, vp, vp]
         L.ti_attn_prefill_set_kernel.argtypes = [i32]
+        if hasattr(L, "ti_paged_append"):
+            cache, attn = C.POINTER(PagedCache), C.POINTER(PagedAttnArgs)
+            L.ti_paged_append.argtypes = [cache, C.POINTER(PagedAppendArgs), vp]
+            L.ti_paged_read.argtypes = [cache, vp, i32, vp, i32, vp, i32, vp]
+            L.ti_paged_workspace_bytes.argtypes = [cache, attn]
+            L.ti_paged_workspace_bytes.restype = sz
+            L.ti_paged_decode.argtypes = L.ti_paged_prefill.argtypes = [cache, attn, vp]
         if hasattr(L, "ti_sample_device"):
             L.ti_sample_device.argtypes = [vp, i32, i32, i32, f32, i32, f32, vp, vp, vp, vp]
         if hasattr(L, "ti_sample_device_ws"):

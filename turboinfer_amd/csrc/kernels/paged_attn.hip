@@ -1,0 +1,457 @@
+// paged_attn.hip -- attention over the paged cache: single tokens and few rows (ti_paged_decode, ti_paged_prefill).
+//
+// o = sum_j w_j v_j / sum_j w_j, w_j = 2^(score_j - m): one pass over the keys, the running reference m moved only where a weight
+// would pass 2^15 (sums follow by 2^(m - m')).
+//
+// 16 columns -- (row, query head) pairs that share a kv-head -- are a tile; a workgroup's four waves take the tile's keys 32 at a
+// time in turn, straight from HBM into registers:
+//   S^T = K Q^T   16x16x32: lane (r = l & 15, g = l >> 4) loads key r of a block of 16; gets the scores of keys 4g .. of column r
+//   O^T += V^T P^T 16x16x32 over two blocks: the lane's own 8 weights are its operand; values: the lane loads dims r D/16 .. of keys
+//                 4g .. of both blocks (whole rows by 16 lanes), byte permutes make 8 keys of one dim of them.
+// So a block's rows come in by whole cache lines, nothing goes through LDS but the waves' sums at the end, and every accumulator
+// belongs to the lane's own column.  Blocks that the table does not have, and rows past the sequence's end, are read through
+// buffer descriptors of their own size: they come in as zeros whatever memory holds, and are masked.
+//
+// int8: score (q . k) ks, ks a block's; weights are taken with the values' scale, 2^(score + log2 vs - m), so that fp16 weights stay
+// near 1 whatever vs, times exact values; the denominator gets them times 1 / vs.  Queries are scaled to fp16 by a power of 2.
+//
+// A tile's keys are cut over workgroups (grid z), by absolute length, and joined by a second launch.
+#include <math.h>
+
+#include "paged_attn.hpp"
+
+namespace ti {
+
+constexpr int kStreamWaves = 4, kStreamKeys = 32;   // keys a wave takes at a time
+
+// Raw keys and values of 32 keys.
+template <int D, bool I8>
+struct StreamRaw {
+  static constexpr int KW = D / (I8 ? 64 : 32), DV = D / 16, VD = DV * (I8 ? 1 : 2) / 4;   // loads a key tile; dims a lane; dwords a key
+  u32x4 k[2][KW];
+  uint32_t v[8][VD];
+};
+
+template <int VD>
+__device__ __forceinline__ void load_dwords(__amdgpu_buffer_rsrc_t rs, int off, uint32_t* to) {
+  if constexpr (VD == 1) {
+    to[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
+  } else if constexpr (VD == 2) {
+    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, 0));
+    to[0] = x[0];
+    to[1] = x[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VD / 4; ++i) {
+      const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off + 16 * i, 0, 0));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[4 * i + j] = x[j];
+    }
+  }
+}
+
+template <int D, class T, bool I8>
+__global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_stream_kernel(const PagedAttn a) {
+  typedef typename PagedMat<T, I8>::M M;
+  typedef typename PagedMat<T, I8>::V8 V8;
+  typedef StreamRaw<D, I8> Raw;
+  constexpr int NK = D / 32, DV = Raw::DV, ES = I8 ? 1 : 2, NW = kStreamWaves;
+  __shared__ float sums[NW][16][D + 4];
+  __shared__ float ml[2][NW][16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.y, split = blockIdx.z, per_seq = (a.G + 15) >> 4;
+  const int b = a.r.start ? paged_find(a.c.seqs, blockIdx.x, [&](int j) { return paged_tile0((long)a.r.start[j] * a.G, j, 16); })
+                          : (int)blockIdx.x / per_seq;
+  if (b >= a.c.seqs) return;
+  const PagedSeq s = paged_seq(a.c, a.r, b);
+  const long tile = a.r.start ? blockIdx.x - paged_tile0((long)s.row0 * a.G, b, 16) : (int)blockIdx.x - b * per_seq;
+  if (tile < 0 || tile * 16 >= (long)s.n * a.G) return;
+  const int ci = (int)tile * 16 + r, row = ci / a.G, head = kvh * a.G + (ci - row * a.G), m = s.row0 + row, p = s.pos0 + row;
+  const bool live = row < s.n && p >= 0 && p < a.c.s.blocks * kPagedBlock;
+  PagedSpan span = {1, 0};
+  if (live) span = paged_span(a, s, m, p);
+  // the tile's keys: any column's, every column's
+  const bool some = span.lo <= span.hi;
+  int lo_any = some ? span.lo : INT32_MAX, hi_any = some ? span.hi : -1, lo_all = live ? span.lo : 0, hi_all = live ? span.hi : INT32_MAX;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    lo_any = min(lo_any, __shfl_xor(lo_any, o, 64));
+    hi_any = max(hi_any, __shfl_xor(hi_any, o, 64));
+    lo_all = max(lo_all, __shfl_xor(lo_all, o, 64));
+    hi_all = min(hi_all, __shfl_xor(hi_all, o, 64));
+  }
+  lo_any = __builtin_amdgcn_readfirstlane(lo_any);
+  hi_any = __builtin_amdgcn_readfirstlane(hi_any);
+  lo_all = __builtin_amdgcn_readfirstlane(lo_all);
+  hi_all = __builtin_amdgcn_readfirstlane(hi_all);
+
+  // queries: 16-bit keys' step c: dims 32 c + 8 g ..; int8: dims 64 (c / 2) + 16 g + 8 (c & 1) ..
+  V8 qf[NK];
+  float f = a.f;
+  {
+    const T* qr = (const T*)a.q + (size_t)m * a.ldq + (size_t)head * D;
+    u16x8 raw[NK];
+#pragma unroll
+    for (int c = 0; c < NK; ++c) {
+      raw[c] = (u16x8){};
+      if (live) raw[c] = *(const u16x8*)(qr + (I8 ? 64 * (c >> 1) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g));
+    }
+    if constexpr (std::is_same_v<M, T>) {
+#pragma unroll
+      for (int c = 0; c < NK; ++c) qf[c] = __builtin_bit_cast(V8, raw[c]);
+    } else {   // bf16 queries as fp16: the column's largest brought to [1, 2), exactly; smaller ones by 2^-24 of it at worst
+      uint32_t top = 0;
+#pragma unroll
+      for (int c = 0; c < NK; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, raw[c][e] & 0x7f80u);
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+      const int ex = (int)(top >> 7) - 127;   // (0, subnormal, infinite: as they are)
+      const bool scaled = top != 0 && top != 0x7f80u;
+      const float up = scaled ? ldexpf(1.0f, -ex) : 1.0f;
+      if (scaled) f = ldexpf(f, ex);
+#pragma unroll
+      for (int c = 0; c < NK; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qf[c][e] = (M)(__builtin_bit_cast(float, (uint32_t)raw[c][e] << 16) * up);
+    }
+  }
+  const float slope = a.slopes && live ? a.slopes[head] * kPagedLog2e : 0.0f;
+
+  f32x4 o[DV];
+#pragma unroll
+  for (int t = 0; t < DV; ++t) o[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float mr = -INFINITY, lr = 0.0f;   // o, lr: relative to 2^mr
+
+  const int step_lo = lo_any >= kStreamKeys ? lo_any / kStreamKeys : 0, step_end = hi_any < 0 ? 0 : hi_any / kStreamKeys + 1;
+  for (int s0 = step_lo + split * a.steps; hi_any >= 0 && s0 < step_end; s0 += a.splits * a.steps) {
+    const int s1 = min(s0 + a.steps, step_end);
+    for (int at = s0 + wave; at < s1; at += 32 * NW) {
+      // lane 2 i + t: block t of the wave's i-th step from here
+      const int my = at + (lane >> 1) * NW, blk = 2 * my + (lane & 1);
+      int id = -1;
+      if (my < s1 && blk < a.c.s.blocks) id = paged_block(a.c.s, a.c.table[(size_t)b * a.c.table_ld + paged_column(a.c.s, blk)], kvh, blk);
+      float ks = 1.0f, vs = 1.0f;
+      if (I8 && id >= 0) {
+        ks = a.c.ks[id];
+        vs = a.c.vs[id];
+        vs = vs < kPagedTiny ? kPagedTiny : vs;
+      }
+      const int n = min(32, (s1 - at + NW - 1) / NW);
+      auto load = [&](int i, Raw& x) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int ib = i < n ? __builtin_amdgcn_readlane(id, 2 * (i & 31) + t) : -1;
+          const int have = ib < 0 ? 0 : min(16, s.len - 16 * (2 * (at + i * NW) + t)) * D * ES;   // (bytes of the block that there are)
+          const size_t off = (size_t)max(ib, 0) * (16 * D * ES);
+          const auto krs = __builtin_amdgcn_make_buffer_rsrc((char*)a.c.k + off, 0, max(have, 0), 0x00020000);
+          const auto vrs = __builtin_amdgcn_make_buffer_rsrc((char*)a.c.v + off, 0, max(have, 0), 0x00020000);
+#pragma unroll
+          for (int c = 0; c < Raw::KW; ++c)
+            x.k[t][c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, r * D * ES + 64 * c + 16 * g, 0, 0));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) load_dwords<Raw::VD>(vrs, ((4 * g + e) * D + r * DV) * ES, x.v[4 * t + e]);
+        }
+      };
+      auto compute = [&](int i, Raw& x) {
+        f32x4 sc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          sc[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < NK; ++c) {
+            u32x4 kw;
+            if constexpr (I8) {
+              const uint32_t w0 = x.k[t][c >> 1][2 * (c & 1)], w1 = x.k[t][c >> 1][2 * (c & 1) + 1];
+              kw = (u32x4){i8_of<false>(w0), i8_of<true>(w0), i8_of<false>(w1), i8_of<true>(w1)};
+            } else {
+              kw = x.k[t][c];
+            }
+            sc[t] = pmma(__builtin_bit_cast(V8, kw), qf[c], sc[t]);
+          }
+        }
+        const int key0 = (at + i * NW) * kStreamKeys;
+        const int id0 = __builtin_amdgcn_readlane(id, 2 * i), id1 = __builtin_amdgcn_readlane(id, 2 * i + 1);
+        const bool ragged = key0 < lo_all || key0 + kStreamKeys - 1 > hi_all || (id0 | id1) < 0;
+        float vl[2] = {0.0f, 0.0f}, vi[2] = {1.0f, 1.0f};
+        float mx = -INFINITY;
+        uint32_t see = 255;
+        if (ragged) {
+          see = 0;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = key0 + 16 * t + 4 * g + e;
+              if (j >= span.lo && j <= span.hi && (t ? id1 : id0) >= 0) see |= 1u << (4 * t + e);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float ft = f;
+          if constexpr (I8) {
+            ft *= __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), 2 * i + t));
+            const float sv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), 2 * i + t));
+            vl[t] = __builtin_amdgcn_logf(sv);
+            vi[t] = ragged && !(see >> 4 * t & 15) ? 0.0f : __builtin_amdgcn_rcpf(sv);   // (0 of a block, whose scale may be NaN)
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = paged_score(sc[t][e], ft, a.cap);
+            if (a.slopes) v = fmaf(slope, (float)(key0 + 16 * t + 4 * g + e - p), v);
+            if constexpr (I8) v += vl[t];
+            if (ragged && !(see >> (4 * t + e) & 1)) v = -INFINITY;
+            sc[t][e] = v;
+            mx = fmaxf(mx, v);
+          }
+        }
+        mx = xor32_max(xor16_max(mx));
+        if (__builtin_amdgcn_ballot_w64(mx > mr + 15.0f) != 0) {
+          const float mn = mx > mr + 15.0f ? mx - 7.0f : mr, alpha = mn == mr ? 1.0f : __builtin_amdgcn_exp2f(mr - mn);
+          mr = mn;
+          lr *= alpha;
+#pragma unroll
+          for (int t = 0; t < DV; ++t) o[t] *= alpha;
+        }
+        const float off = mr == -INFINITY ? 0.0f : mr;
+        V8 pf;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float l = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float w = __builtin_amdgcn_exp2f(sc[t][e] - off);
+            l += w;
+            pf[4 * t + e] = (M)w;
+          }
+          lr = fmaf(l, vi[t], lr);
+        }
+        // 8 keys of dims r DV + t: the values' operand
+        auto frag = [&](int t) {
+          u32x4 vw;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (I8) {
+              const uint32_t sel = 0x0c000c00u | (uint32_t)(t & 3) | (uint32_t)(4 + (t & 3)) << 16;
+              vw[e] = i8_pair(__builtin_amdgcn_perm(x.v[2 * e + 1][t >> 2], x.v[2 * e][t >> 2], sel));
+            } else {
+              vw[e] = __builtin_amdgcn_perm(x.v[2 * e + 1][t >> 1], x.v[2 * e][t >> 1], t & 1 ? 0x07060302u : 0x05040100u);
+            }
+          }
+          return vw;
+        };
+        if constexpr (!I8)
+          if (ragged) {
+            typedef PagedOdd<M> Odd;
+            uint32_t bad = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+              for (int w = 0; w < Raw::VD; ++w) bad |= Odd::any(x.v[e][w]);
+            if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+              const V8 one = Odd::seen(see);
+#pragma unroll
+              for (int t = 0; t < DV; ++t) o[t] = Odd::add(frag(t), one, o[t]);
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int w = 0; w < Raw::VD; ++w) x.v[e][w] = Odd::finite(x.v[e][w]);
+            }
+          }
+#pragma unroll
+        for (int t = 0; t < DV; ++t) o[t] = pmma(__builtin_bit_cast(V8, frag(t)), pf, o[t]);
+      };
+      Raw x0, x1;
+      load(0, x0);
+      for (int i = 0; i < n; i += 2) {
+        load(i + 1, x1);
+        compute(i, x0);
+        load(i + 2, x0);
+        if (i + 1 < n) compute(i + 1, x1);
+      }
+    }
+  }
+  lr += lane_xor<16>(lr);
+  lr += lane_xor<32>(lr);
+  // the waves' sums: dims (4 g + i) DV + t of column r
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int t = 0; t < DV; ++t) sums[wave][r][(4 * g + i) * DV + t] = o[t][i];
+  if (g == 0) {
+    ml[0][wave][r] = mr;
+    ml[1][wave][r] = lr;
+  }
+  __syncthreads();
+  const int col = threadIdx.x >> 4, part = threadIdx.x & 15;   // thread: dims part * DV .. of column col
+  const int cj = (int)tile * 16 + col, row_c = cj / a.G, head_c = kvh * a.G + (cj - row_c * a.G), p_c = s.pos0 + row_c;
+  if (row_c >= s.n || p_c < 0 || p_c >= a.c.s.blocks * kPagedBlock) return;
+  float mm = -INFINITY, l = 0.0f, w[NW];
+#pragma unroll
+  for (int i = 0; i < NW; ++i) mm = fmaxf(mm, ml[0][i][col]);
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const float mi = ml[0][i][col];
+    w[i] = mi == -INFINITY && ml[1][i][col] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mi - mm);
+    l += ml[1][i][col] * w[i];
+  }
+  float acc[DV];
+#pragma unroll
+  for (int d = 0; d < DV; ++d) {
+    acc[d] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i)
+      if (w[i] != 0.0f) acc[d] += w[i] * sums[i][col][part * DV + d];
+  }
+  const size_t rh = (size_t)(s.row0 + row_c) * a.heads + head_c;
+  if (a.splits > 1) {
+    const size_t at = rh * a.splits + split;
+    if (part == 0) *(float2*)(a.part_ml + 2 * at) = make_float2(mm, l);
+    float* po = a.part_o + at * D + part * DV;
+#pragma unroll
+    for (int d = 0; d < DV; d += 4) *(f32x4*)(po + d) = (f32x4){acc[d], acc[d + 1], acc[d + 2], acc[d + 3]};
+    return;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* out = (T*)a.out + (size_t)(s.row0 + row_c) * a.ldo + (size_t)head_c * D + part * DV;
+#pragma unroll
+  for (int d = 0; d < DV; d += 4) {
+    typedef T Q4 __attribute__((ext_vector_type(4)));
+    Q4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (T)(l == 0.0f ? 0.0f : acc[d + e] * inv);
+    *(Q4*)(out + d) = y;
+  }
+}
+
+// A wave a (row, head): the splits' sums joined.  Grid (rows, heads / 4, rounded up).
+template <int D, class T>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn a) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63, m = blockIdx.x, head = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (head >= a.heads) return;
+  const int b = a.r.start ? paged_find(a.c.seqs, m, [&](int j) { return (long)a.r.start[j]; }) : m;
+  if (b >= a.c.seqs) return;
+  const PagedSeq s = paged_seq(a.c, a.r, b);
+  const int p = s.pos0 + (m - s.row0);
+  if (m < s.row0 || m >= s.row0 + s.n || p < 0 || p >= a.c.s.blocks * kPagedBlock) return;
+  const size_t at = ((size_t)m * a.heads + head) * a.splits;
+  float mm = -INFINITY;
+  for (int i = lane; i < a.splits; i += 64) mm = fmaxf(mm, a.part_ml[2 * (at + i)]);
+  mm = wave_max(mm);
+  float l = 0.0f, acc[E] = {};
+  for (int i0 = 0; i0 < a.splits; i0 += 64) {
+    float w = 0.0f;
+    if (i0 + lane < a.splits) {
+      const float2 x = *(const float2*)(a.part_ml + 2 * (at + i0 + lane));
+      w = x.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x.x - mm);
+      l += x.y * w;
+    }
+    const int n = min(64, a.splits - i0);
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      float x[8][E], wj[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        wj[j] = j0 + j < n ? __shfl(w, j0 + j, 64) : 0.0f;
+        const float* po = a.part_o + (at + min(i0 + j0 + j, a.splits - 1)) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[j][e] = po[e];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (wj[j] != 0.0f)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(wj[j], x[j][e], acc[e]);
+    }
+  }
+  l = group_sum<64>(l);
+  T* out = (T*)a.out + (size_t)m * a.ldo + (size_t)head * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[e] = (T)(l == 0.0f ? 0.0f : acc[e] / l);
+}
+
+// Splits of a call's keys: enough workgroups for the CUs.
+struct StreamPlan {
+  long tiles;
+  int splits, steps, most;   // most: splits of any length
+};
+static StreamPlan stream_plan(const ti_paged_cache* c, const ti_paged_attn_args* p) {
+  const int G = p->heads / c->kv_heads;
+  const long tiles = p->row_start ? paged_tiles((long)p->rows * G, c->seqs, 16) : (long)c->seqs * ((G + 15) / 16);
+  long span = (long)c->table_ld * c->page;
+  if (p->max_len > 0) span = std::min<long>(span, p->max_len);
+  if (p->window > 0 && !p->prefix) span = std::min<long>(span, (long)p->window + 16);
+  const long steps = (span + kStreamKeys - 1) / kStreamKeys, units = std::max(1l, tiles * c->kv_heads);
+  const long most = std::min((1024 + units - 1) / units, 256l);
+  const long splits = std::max(1l, std::min(most, (steps + kStreamWaves - 1) / kStreamWaves));
+  const int per = (int)(((steps + splits - 1) / splits + kStreamWaves - 1) / kStreamWaves * kStreamWaves);
+  return {tiles, (int)std::max(1l, (steps + per - 1) / per), per, (int)most};
+}
+
+template <int D, class T>
+int stream(PagedAttn a, const StreamPlan& plan, const ti_paged_cache* c, hipStream_t s) {
+  const dim3 grid((unsigned)plan.tiles, c->kv_heads, plan.splits);
+  if (c->kv_type == TI_KV_I8)
+    hipLaunchKernelGGL((paged_stream_kernel<D, T, true>), grid, dim3(64 * kStreamWaves), 0, s, a);
+  else
+    hipLaunchKernelGGL((paged_stream_kernel<D, T, false>), grid, dim3(64 * kStreamWaves), 0, s, a);
+  TI_LAUNCH_CHECK("paged_stream_kernel");
+  if (plan.splits > 1) {
+    hipLaunchKernelGGL((paged_join_kernel<D, T>), dim3(a.r.rows, (a.heads + 3) / 4), dim3(256), 0, s, a);
+    TI_LAUNCH_CHECK("paged_join_kernel");
+  }
+  return TI_OK;
+}
+
+static size_t part_bytes(const ti_paged_cache* c, const ti_paged_attn_args* p, int splits) {
+  return splits < 2 ? 0 : (size_t)p->rows * p->heads * splits * ((size_t)c->head_dim + 2) * sizeof(float);
+}
+
+static int check_attn(const ti_paged_cache* c, const ti_paged_attn_args* p, const char* who) {
+  if (const int rc = ti_paged_check(c, who)) return rc;
+  if (!p) return ti_set_error(TI_ERR_ARG, "%s: null arguments", who);
+  if (p->rows < 0 || p->rows > (1 << 24) || p->heads < 1 || p->heads > 16384 || p->heads % c->kv_heads || p->max_len < 0 || p->window < 0)
+    return ti_set_error(TI_ERR_ARG, "%s: bad sizes rows=%d heads=%d kv_heads=%d max_len=%d window=%d", who, p->rows, p->heads, c->kv_heads,
+                        p->max_len, p->window);
+  if (!p->row_start && p->rows != c->seqs) return ti_set_error(TI_ERR_ARG, "%s: %d rows of %d sequences without row_start", who, p->rows, c->seqs);
+  if (!(p->softcap >= 0.0f) || !(p->softcap < 3e38f) || !(fabsf(p->scale) < 3e38f))
+    return ti_set_error(TI_ERR_ARG, "%s: scale %g, softcap %g", who, (double)p->scale, (double)p->softcap);
+  return TI_OK;
+}
+
+static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_stream_t stream_, const char* who) {
+  if (const int rc = check_attn(c, p, who)) return rc;
+  if (!p->q || !p->out) return ti_set_error(TI_ERR_ARG, "%s: null pointer", who);
+  const int64_t w = (int64_t)p->heads * c->head_dim;
+  if (p->ldq < w || p->ldo < w || p->ldq % 8 || p->ldo % 8 || ((uintptr_t)p->q | (uintptr_t)p->out) % 16)
+    return ti_set_error(TI_ERR_ARG, "%s: rows of pitch %d, %d for %ld values, or not 16-byte aligned", who, p->ldq, p->ldo, (long)w);
+  if (((uintptr_t)p->row_start | (uintptr_t)p->slopes | (uintptr_t)p->first | (uintptr_t)p->prefix) % 4 || (uintptr_t)p->workspace % 16)
+    return ti_set_error(TI_ERR_ARG, "%s: pointers are not aligned", who);
+  if (p->rows == 0) return TI_OK;
+  const StreamPlan plan = stream_plan(c, p);
+  const size_t need = part_bytes(c, p, plan.splits);
+  if (need && (!p->workspace || p->workspace_bytes < (int64_t)need))
+    return ti_set_error(TI_ERR_ARG, "%s: workspace of %ld bytes, %zu needed", who, (long)(p->workspace ? p->workspace_bytes : 0), need);
+  const size_t n_o = (size_t)p->rows * p->heads * plan.splits * c->head_dim;
+  float* ws = (float*)p->workspace;
+  const float cap = p->softcap;
+  const PagedAttn a = {ti_paged_form(c), {p->row_start, p->rows}, p->q, p->out, p->slopes, p->first, p->prefix, ws, need ? ws + n_o : nullptr,
+                       p->heads, p->heads / c->kv_heads, p->ldq, p->ldo, p->window, plan.splits, plan.steps,
+                       cap > 0.0f ? 2.0f * p->scale * kPagedLog2e / cap : p->scale * kPagedLog2e, cap * kPagedLog2e};
+  return TI_PAGED_FORM(c, stream, a, plan, c, (hipStream_t)stream_);
+}
+
+}  // namespace ti
+
+extern "C" size_t ti_paged_workspace_bytes(const ti_paged_cache* c, const ti_paged_attn_args* a) {
+  if (ti::check_attn(c, a, "ti_paged_workspace_bytes")) return 0;
+  return ti::part_bytes(c, a, ti::stream_plan(c, a).most);
+}
+
+extern "C" int ti_paged_decode(const ti_paged_cache* c, const ti_paged_attn_args* a, ti_stream_t s) {
+  if (a && a->row_start) return ti_set_error(TI_ERR_ARG, "ti_paged_decode: row_start (rows of several tokens: ti_paged_prefill)");
+  return ti::attend(c, a, s, "ti_paged_decode");
+}
+
+extern "C" int ti_paged_prefill(const ti_paged_cache* c, const ti_paged_attn_args* a, ti_stream_t s) { return ti::attend(c, a, s, "ti_paged_prefill"); }

@@ -1,0 +1,74 @@
+// paged_device.hpp -- what the kernels of the paged cache share (paged_cache.hip, paged_attn.hip).
+#pragma once
+
+#include "elem.hpp"
+#include "paged.hpp"
+
+namespace ti {
+
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+struct PagedCache {
+  void* k;
+  void* v;
+  float* ks;
+  float* vs;
+  const int32_t* table;
+  const int32_t* len;
+  int table_ld, seqs;
+  PagedShape s;
+};
+
+// Ragged rows: where the sequences' rows start (NULL: row b is sequence b's).
+struct PagedRows {
+  const int32_t* start;
+  int rows;
+};
+__device__ __forceinline__ int paged_start(const PagedRows& r, int b) { return r.start ? r.start[b] : b; }
+
+// The last sequence whose first tile (row, ..: key(b), not falling) is at most i, by one wave: the number of b in 1 .. seqs - 1 with
+// key(b) <= i.
+template <class Key>
+__device__ __forceinline__ int paged_find(int seqs, long i, Key key) {
+  const int lane = threadIdx.x & 63;
+  int b = 0;
+  for (int b0 = 1; b0 < seqs; b0 += 64) {
+    const int n = __popcll(__builtin_amdgcn_ballot_w64(b0 + lane < seqs && key(b0 + lane) <= i));
+    b += n;
+    if (n < 64) break;
+  }
+  return __builtin_amdgcn_readfirstlane(b);
+}
+
+// A sequence's rows: row0 .. row0 + n - 1 of the call, tokens pos0 ..; len: its keys, within the table.
+struct PagedSeq {
+  int b, row0, n, pos0, len;
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedCache& c, const PagedRows& r, int b) {
+  const int r0 = max(paged_start(r, b), 0), r1 = min(paged_start(r, b + 1), r.rows), n = max(r1 - r0, 0);
+  const int len = c.len[b], most = c.s.blocks * kPagedBlock;
+  return {b, r0, n, (int)max((long)len - n, (long)INT32_MIN / 2), min(max(len, 0), most)};
+}
+
+// Values of a 16-bit type.
+template <class T>
+__device__ __forceinline__ u16x8 pack8(const float* v) {
+  typedef T V __attribute__((ext_vector_type(8)));
+  V o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = (T)v[e];
+  return __builtin_bit_cast(u16x8, o);
+}
+
+}  // namespace ti
+
+// fn<D, T>(args ..) of the cache's sizes
+#define TI_PAGED_FORM(c, fn, ...)                                                                                     \
+  ((c)->dtype == TI_PAGED_F16                                                                                        \
+       ? (c)->head_dim == 64 ? fn<64, f16>(__VA_ARGS__) : (c)->head_dim == 128 ? fn<128, f16>(__VA_ARGS__) : fn<256, f16>(__VA_ARGS__) \
+       : (c)->head_dim == 64 ? fn<64, bf16>(__VA_ARGS__) : (c)->head_dim == 128 ? fn<128, bf16>(__VA_ARGS__) : fn<256, bf16>(__VA_ARGS__))
+
+// Checks of a cache's description (TI_OK, or the error set), and its kernels' form.
+extern "C++" int ti_paged_check(const ti_paged_cache* c, const char* who);
+extern "C++" ti::PagedCache ti_paged_form(const ti_paged_cache* c);

@@ -1,4 +1,5 @@
-// paged_attn.hip -- attention over the paged cache: single tokens and few rows (ti_paged_decode, ti_paged_prefill).
+// paged_attn.hip -- attention over the paged cache: single tokens and few rows (ti_paged_decode, ti_paged_prefill; many rows:
+// paged_prefill.hip).
 //
 // o = sum_j w_j v_j / sum_j w_j, w_j = 2^(score_j - m): one pass over the keys, the running reference m moved only where a weight
 // would pass 2^15 (sums follow by 2^(m - m')).
@@ -371,32 +372,45 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn a) {
   for (int e = 0; e < E; ++e) out[e] = (T)(l == 0.0f ? 0.0f : acc[e] / l);
 }
 
-// Splits of a call's keys: enough workgroups for the CUs.
-struct StreamPlan {
+// A call's kernel and splits of its keys: enough workgroups for the CUs.
+struct PagedPlan {
+  bool block;   // paged_prefill.hip
   long tiles;
   int splits, steps, most;   // most: splits of any length
 };
-static StreamPlan stream_plan(const ti_paged_cache* c, const ti_paged_attn_args* p) {
+static PagedPlan paged_plan(const ti_paged_cache* c, const ti_paged_attn_args* p) {
   const int G = p->heads / c->kv_heads;
-  const long tiles = p->row_start ? paged_tiles((long)p->rows * G, c->seqs, 16) : (long)c->seqs * ((G + 15) / 16);
+  const long columns = (long)p->rows * G;
+  const bool block = p->row_start && columns >= 64l * c->seqs;
+  const int cols = block ? paged_block_cols(c->head_dim) : 16;
+  const long tiles = p->row_start ? paged_tiles(columns, c->seqs, cols) : (long)c->seqs * ((G + 15) / 16);
   long span = (long)c->table_ld * c->page;
   if (p->max_len > 0) span = std::min<long>(span, p->max_len);
-  if (p->window > 0 && !p->prefix) span = std::min<long>(span, (long)p->window + 16);
-  const long steps = (span + kStreamKeys - 1) / kStreamKeys, units = std::max(1l, tiles * c->kv_heads);
+  if (p->window > 0 && !p->prefix) span = std::min<long>(span, (long)p->window + cols);
+  const long units = std::max(1l, tiles * c->kv_heads);
+  if (block) {
+    const long steps = (span + 63) / 64, most = std::max(1l, std::min(256 / units, 64l));
+    return {true, tiles, (int)std::max(1l, std::min(most, steps / 8)), 0, (int)most};
+  }
+  const long steps = (span + kStreamKeys - 1) / kStreamKeys;
   const long most = std::min((1024 + units - 1) / units, 256l);
   const long splits = std::max(1l, std::min(most, (steps + kStreamWaves - 1) / kStreamWaves));
   const int per = (int)(((steps + splits - 1) / splits + kStreamWaves - 1) / kStreamWaves * kStreamWaves);
-  return {tiles, (int)std::max(1l, (steps + per - 1) / per), per, (int)most};
+  return {false, tiles, (int)std::max(1l, (steps + per - 1) / per), per, (int)most};
 }
 
 template <int D, class T>
-int stream(PagedAttn a, const StreamPlan& plan, const ti_paged_cache* c, hipStream_t s) {
-  const dim3 grid((unsigned)plan.tiles, c->kv_heads, plan.splits);
-  if (c->kv_type == TI_KV_I8)
-    hipLaunchKernelGGL((paged_stream_kernel<D, T, true>), grid, dim3(64 * kStreamWaves), 0, s, a);
-  else
-    hipLaunchKernelGGL((paged_stream_kernel<D, T, false>), grid, dim3(64 * kStreamWaves), 0, s, a);
-  TI_LAUNCH_CHECK("paged_stream_kernel");
+int launch_attn(PagedAttn a, const PagedPlan& plan, const ti_paged_cache* c, hipStream_t s) {
+  if (plan.block) {
+    if (const int rc = paged_block(a, c, plan.tiles, s)) return rc;
+  } else {
+    const dim3 grid((unsigned)plan.tiles, c->kv_heads, plan.splits);
+    if (c->kv_type == TI_KV_I8)
+      hipLaunchKernelGGL((paged_stream_kernel<D, T, true>), grid, dim3(64 * kStreamWaves), 0, s, a);
+    else
+      hipLaunchKernelGGL((paged_stream_kernel<D, T, false>), grid, dim3(64 * kStreamWaves), 0, s, a);
+    TI_LAUNCH_CHECK("paged_stream_kernel");
+  }
   if (plan.splits > 1) {
     hipLaunchKernelGGL((paged_join_kernel<D, T>), dim3(a.r.rows, (a.heads + 3) / 4), dim3(256), 0, s, a);
     TI_LAUNCH_CHECK("paged_join_kernel");
@@ -415,6 +429,7 @@ static int check_attn(const ti_paged_cache* c, const ti_paged_attn_args* p, cons
     return ti_set_error(TI_ERR_ARG, "%s: bad sizes rows=%d heads=%d kv_heads=%d max_len=%d window=%d", who, p->rows, p->heads, c->kv_heads,
                         p->max_len, p->window);
   if (!p->row_start && p->rows != c->seqs) return ti_set_error(TI_ERR_ARG, "%s: %d rows of %d sequences without row_start", who, p->rows, c->seqs);
+  if ((int64_t)p->rows * p->heads > INT32_MAX) return ti_set_error(TI_ERR_ARG, "%s: %d rows of %d heads in a call", who, p->rows, p->heads);
   if (!(p->softcap >= 0.0f) || !(p->softcap < 3e38f) || !(fabsf(p->scale) < 3e38f))
     return ti_set_error(TI_ERR_ARG, "%s: scale %g, softcap %g", who, (double)p->scale, (double)p->softcap);
   return TI_OK;
@@ -429,7 +444,7 @@ static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_strea
   if (((uintptr_t)p->row_start | (uintptr_t)p->slopes | (uintptr_t)p->first | (uintptr_t)p->prefix) % 4 || (uintptr_t)p->workspace % 16)
     return ti_set_error(TI_ERR_ARG, "%s: pointers are not aligned", who);
   if (p->rows == 0) return TI_OK;
-  const StreamPlan plan = stream_plan(c, p);
+  const PagedPlan plan = paged_plan(c, p);
   const size_t need = part_bytes(c, p, plan.splits);
   if (need && (!p->workspace || p->workspace_bytes < (int64_t)need))
     return ti_set_error(TI_ERR_ARG, "%s: workspace of %ld bytes, %zu needed", who, (long)(p->workspace ? p->workspace_bytes : 0), need);
@@ -439,14 +454,14 @@ static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_strea
   const PagedAttn a = {ti_paged_form(c), {p->row_start, p->rows}, p->q, p->out, p->slopes, p->first, p->prefix, ws, need ? ws + n_o : nullptr,
                        p->heads, p->heads / c->kv_heads, p->ldq, p->ldo, p->window, plan.splits, plan.steps,
                        cap > 0.0f ? 2.0f * p->scale * kPagedLog2e / cap : p->scale * kPagedLog2e, cap * kPagedLog2e};
-  return TI_PAGED_FORM(c, stream, a, plan, c, (hipStream_t)stream_);
+  return TI_PAGED_FORM(c, launch_attn, a, plan, c, (hipStream_t)stream_);
 }
 
 }  // namespace ti
 
 extern "C" size_t ti_paged_workspace_bytes(const ti_paged_cache* c, const ti_paged_attn_args* a) {
   if (ti::check_attn(c, a, "ti_paged_workspace_bytes")) return 0;
-  return ti::part_bytes(c, a, ti::stream_plan(c, a).most);
+  return ti::part_bytes(c, a, ti::paged_plan(c, a).most);
 }
 
 extern "C" int ti_paged_decode(const ti_paged_cache* c, const ti_paged_attn_args* a, ti_stream_t s) {

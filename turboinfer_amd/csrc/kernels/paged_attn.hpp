@@ -81,14 +81,19 @@ struct PagedOdd {
     for (int i = 0; i < 4; ++i) w[i] = (see >> 2 * i & 1) * kOne | (see >> (2 * i + 1) & 1) * (kOne << 16);
     return __builtin_bit_cast(V8, w);
   }
+  // 1 in the places of +inf or NaN, of -inf or NaN
+  static __device__ __forceinline__ u32x2 signs(uint32_t x) {
+    const uint32_t n = any(x) >> 15, neg = x >> 15 & 0x00010001u, nan = ((x & kMan) + kMan) >> kBits & 0x00010001u;
+    return (u32x2){(n & (~neg | nan)) * kOne, (n & (neg | nan)) * kOne};
+  }
   // acc + what the fragment v's infinities and NaN come to
   static __device__ __forceinline__ f32x4 add(u32x4 v, V8 one, f32x4 acc) {
-    u32x4 up, down;   // +inf or NaN, -inf or NaN
+    u32x4 up, down;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t n = any(v[i]) >> 15, neg = v[i] >> 15 & 0x00010001u, nan = ((v[i] & kMan) + kMan) >> kBits & 0x00010001u;
-      up[i] = (n & (~neg | nan)) * kOne;
-      down[i] = (n & (neg | nan)) * kOne;
+      const u32x2 n = signs(v[i]);
+      up[i] = n[0];
+      down[i] = n[1];
     }
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f}, n_up = pmma(__builtin_bit_cast(V8, up), one, zero), n_down = pmma(__builtin_bit_cast(V8, down), one, zero);
 #pragma unroll
@@ -99,5 +104,9 @@ struct PagedOdd {
     return acc;
   }
 };
+
+// The kernel of many rows (paged_prefill.hip): columns of its tiles, and a launch of `tiles` of them a kv-head.
+int paged_block_cols(int head_dim);
+int paged_block(const PagedAttn& a, const ti_paged_cache* c, long tiles, hipStream_t s);
 
 }  // namespace ti

@@ -51,22 +51,23 @@ __device__ __forceinline__ void load_dwords(__amdgpu_buffer_rsrc_t rs, int off, 
   }
 }
 
+template <int D>
+struct StreamLds {
+  float sums[kStreamWaves][16][D + 4], ml[2][kStreamWaves][16];
+};
+
+// One tile of a sequence over some of its keys: steps u0 .. u1 - 1 of 32, counted from the tile's first (u1 < 0: split u0's part of all).
+// Sums go to part `at` of a row's head, or (a.splits 1) the result to `out`.
 template <int D, class T, bool I8>
-__global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_stream_kernel(const PagedAttn a) {
+__device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_lds, const PagedSeq& s, long tile, int kvh, int u0, int u1, long slot) {
   typedef typename PagedMat<T, I8>::M M;
   typedef typename PagedMat<T, I8>::V8 V8;
   typedef StreamRaw<D, I8> Raw;
   constexpr int NK = D / 32, DV = Raw::DV, ES = I8 ? 1 : 2, NW = kStreamWaves;
-  __shared__ float sums[NW][16][D + 4];
-  __shared__ float ml[2][NW][16];
+  auto& sums = x_lds.sums;
+  auto& ml = x_lds.ml;
+  const int b = s.b;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y, split = blockIdx.z, per_seq = (a.G + 15) >> 4;
-  const int b = a.r.start ? paged_find(a.c.seqs, blockIdx.x, [&](int j) { return paged_tile0((long)a.r.start[j] * a.G, j, 16); })
-                          : (int)blockIdx.x / per_seq;
-  if (b >= a.c.seqs) return;
-  const PagedSeq s = paged_seq(a.c, a.r, b);
-  const long tile = a.r.start ? blockIdx.x - paged_tile0((long)s.row0 * a.G, b, 16) : (int)blockIdx.x - b * per_seq;
-  if (tile < 0 || tile * 16 >= (long)s.n * a.G) return;
   const int ci = (int)tile * 16 + r, row = ci / a.G, head = kvh * a.G + (ci - row * a.G), m = s.row0 + row, p = s.pos0 + row;
   const bool live = row < s.n && p >= 0 && p < a.c.s.blocks * kPagedBlock;
   PagedSpan span = {1, 0};
@@ -125,9 +126,14 @@ __global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_str
   for (int t = 0; t < DV; ++t) o[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
   float mr = -INFINITY, lr = 0.0f;   // o, lr: relative to 2^mr
 
-  const int step_lo = lo_any >= kStreamKeys ? lo_any / kStreamKeys : 0, step_end = hi_any < 0 ? 0 : hi_any / kStreamKeys + 1;
-  for (int s0 = step_lo + split * a.steps; hi_any >= 0 && s0 < step_end; s0 += a.splits * a.steps) {
-    const int s1 = min(s0 + a.steps, step_end);
+  const int step_lo = hi_any < 0 ? 0 : lo_any / kStreamKeys, n_steps = hi_any < 0 ? 0 : hi_any / kStreamKeys + 1 - step_lo;
+  if (u1 < 0) {
+    const int each = (n_steps + a.splits - 1) / a.splits;
+    u0 *= each;
+    u1 = u0 + each;
+  }
+  const int s0 = step_lo + u0, s1 = step_lo + min(u1, n_steps);
+  {
     for (int at = s0 + wave; at < s1; at += 32 * NW) {
       // lane 2 i + t: block t of the wave's i-th step from here
       const int my = at + (lane >> 1) * NW, blk = 2 * my + (lane & 1);
@@ -179,13 +185,15 @@ __global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_str
         float mx = -INFINITY;
         uint32_t see = 255;
         if (ragged) {
+          int lo = span.lo;
+          asm volatile("" : "+v"(lo));   // (a branch, not selects: most steps skip it)
           see = 0;
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = key0 + 16 * t + 4 * g + e;
-              if (j >= span.lo && j <= span.hi && (t ? id1 : id0) >= 0) see |= 1u << (4 * t + e);
+              if (j >= lo && j <= span.hi && (t ? id1 : id0) >= 0) see |= 1u << (4 * t + e);
             }
         }
 #pragma unroll
@@ -197,15 +205,32 @@ __global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_str
             vl[t] = __builtin_amdgcn_logf(sv);
             vi[t] = ragged && !(see >> 4 * t & 15) ? 0.0f : __builtin_amdgcn_rcpf(sv);   // (0 of a block, whose scale may be NaN)
           }
+          if (a.cap != 0.0f) {
+            float cap = a.cap;
+            asm volatile("" : "+s"(cap));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float v = paged_score(sc[t][e], ft, a.cap);
-            if (a.slopes) v = fmaf(slope, (float)(key0 + 16 * t + 4 * g + e - p), v);
-            if constexpr (I8) v += vl[t];
-            if (ragged && !(see >> (4 * t + e) & 1)) v = -INFINITY;
-            sc[t][e] = v;
-            mx = fmaxf(mx, v);
+            for (int e = 0; e < 4; ++e) sc[t][e] = paged_capped(sc[t][e], ft, cap);
+            ft = 1.0f;
           }
+          if (a.slopes) {
+            float slope_ = slope;
+            asm volatile("" : "+v"(slope_));
+            const float base = fmaf(slope_, (float)(key0 + 16 * t + 4 * g - p), vl[t]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[t][e] = fmaf(sc[t][e], ft, fmaf(slope_, (float)e, base));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[t][e] = I8 ? fmaf(sc[t][e], ft, vl[t]) : sc[t][e] * ft;
+          }
+          if (ragged) {
+            uint32_t have = see;
+            asm volatile("" : "+v"(have));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!(have >> (4 * t + e) & 1)) sc[t][e] = -INFINITY;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][e]);
         }
         mx = xor32_max(xor16_max(mx));
         if (__builtin_amdgcn_ballot_w64(mx > mr + 15.0f) != 0) {
@@ -305,9 +330,8 @@ __global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_str
     for (int i = 0; i < NW; ++i)
       if (w[i] != 0.0f) acc[d] += w[i] * sums[i][col][part * DV + d];
   }
-  const size_t rh = (size_t)(s.row0 + row_c) * a.heads + head_c;
-  if (a.splits > 1) {
-    const size_t at = rh * a.splits + split;
+  if (a.part_o) {
+    const size_t at = a.deal ? (size_t)head_c * (a.deal + a.c.seqs) + slot : ((size_t)(s.row0 + row_c) * a.heads + head_c) * a.splits + slot;
     if (part == 0) *(float2*)(a.part_ml + 2 * at) = make_float2(mm, l);
     float* po = a.part_o + at * D + part * DV;
 #pragma unroll
@@ -326,57 +350,158 @@ __global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_str
   }
 }
 
-// A wave a (row, head): the splits' sums joined.  Grid (rows, heads / 4, rounded up).
+// Grid (tiles, kv-heads, splits).
+template <int D, class T, bool I8>
+__global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_stream_kernel(const PagedAttn a) {
+  __shared__ StreamLds<D> lds;
+  const int per_seq = (a.G + 15) >> 4;
+  const int b = a.r.start ? paged_find(a.c.seqs, blockIdx.x, [&](int j) { return paged_tile0((long)a.r.start[j] * a.G, j, 16); })
+                          : (int)blockIdx.x / per_seq;
+  const PagedSeq s = paged_seq(a.c, a.r, b);
+  const long tile = a.r.start ? blockIdx.x - paged_tile0((long)s.row0 * a.G, b, 16) : (int)blockIdx.x - b * per_seq;
+  if (tile < 0 || tile * 16 >= (long)s.n * a.G) return;
+  stream_tile<D, T, I8>(a, lds, s, tile, blockIdx.y, blockIdx.z, -1, blockIdx.z);
+}
+
+// Single tokens: steps of 32 keys that sequence b's row sees.
+__device__ __forceinline__ int decode_steps(const PagedAttn& a, int b) {
+  const int len = a.c.len[b], p = len - 1;
+  if (p < 0 || p >= a.c.s.blocks * kPagedBlock) return 0;
+  int lo = a.window > 0 ? max(p - a.window + 1, 0) : 0;
+  if (a.first) lo = max(lo, a.first[b]);
+  return lo > p ? 0 : p / kStreamKeys - lo / kStreamKeys + 1;
+}
+__device__ __forceinline__ long uniform(long v) {
+  return (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+// Sum over this lane and those in front of it.  (64 sequences of at most 2^26 steps: 32 bits unsigned.)
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+constexpr int kDealLeast = kStreamWaves;   // steps of a run: one a wave
+__device__ __forceinline__ long deal_run(const PagedAttn& a, long all) { return max((all + a.deal - 1) / a.deal, (long)kDealLeast); }
+
+// The steps of all sequences are one list, cut into equal runs for the a.deal workgroups of a kv-head: grid (a.deal, kv-heads * tiles of 16
+// query heads).  Part w + b of a head is workgroup w's of sequence b: each differs from the one in front by 1 in
+// w or more in b.
+template <int D, class T, bool I8>
+__global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_deal_kernel(const PagedAttn a) {
+  __shared__ StreamLds<D> lds;
+  const int lane = threadIdx.x & 63, w = blockIdx.x, per_seq = (a.G + 15) >> 4, kvh = blockIdx.y / per_seq, tile = blockIdx.y - kvh * per_seq;
+  int mine = lane < a.c.seqs ? decode_steps(a, lane) : 0;
+  unsigned sum = wave_scan(mine);
+  long all = (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
+  for (int b0 = 64; b0 < a.c.seqs; b0 += 64)
+    all += (unsigned)__builtin_amdgcn_readlane((int)wave_scan(b0 + lane < a.c.seqs ? decode_steps(a, b0 + lane) : 0), 63);
+  const long per = uniform(deal_run(a, all)), from = w * per, to = from + per;
+  if (from >= all) return;
+  // the sequence that step `from` is in
+  long base = 0;   // steps in front of b
+  int b = 0, n = 0;
+  for (int b0 = 0;;) {
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(base + sum > from);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      b = b0 + l;
+      n = __builtin_amdgcn_readlane(mine, l);
+      base += (unsigned)__builtin_amdgcn_readlane((int)sum, l) - (unsigned)n;
+      break;
+    }
+    base += (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
+    b0 += 64;
+    if (b0 >= a.c.seqs) return;
+    mine = b0 + lane < a.c.seqs ? decode_steps(a, b0 + lane) : 0;
+    sum = wave_scan(mine);
+  }
+  base = uniform(base);
+  for (; n > 0; n = b < a.c.seqs ? __builtin_amdgcn_readfirstlane(decode_steps(a, b)) : 0) {
+    stream_tile<D, T, I8>(a, lds, paged_seq(a.c, a.r, b), tile, kvh, (int)(max(from, base) - base), (int)min((long)n, to - base), (long)w + b);
+    base += n;
+    if (base >= to) break;
+    do ++b;
+    while (b < a.c.seqs && __builtin_amdgcn_readfirstlane(decode_steps(a, b)) == 0);
+    __syncthreads();
+  }
+}
+
+// A workgroup a (row, head): its parts joined, four waves in turn.
 template <int D, class T>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn a) {
   constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63, m = blockIdx.x, head = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (head >= a.heads) return;
+  __shared__ float sums[4][D], ls[4];
+  const int lane = threadIdx.x & 63, m = blockIdx.x, head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = a.r.start ? paged_find(a.c.seqs, m, [&](int j) { return (long)a.r.start[j]; }) : m;
-  if (b >= a.c.seqs) return;
   const PagedSeq s = paged_seq(a.c, a.r, b);
   const int p = s.pos0 + (m - s.row0);
   if (m < s.row0 || m >= s.row0 + s.n || p < 0 || p >= a.c.s.blocks * kPagedBlock) return;
-  const size_t at = ((size_t)m * a.heads + head) * a.splits;
+  size_t at = ((size_t)m * a.heads + head) * a.splits;
+  int n = a.splits;
+  if (a.deal) {
+    long all = 0, before = 0;   // steps of all sequences, of those in front of b
+    int own = 0;
+    for (int b0 = 0; b0 < a.c.seqs; b0 += 64) {
+      const int mine = b0 + lane < a.c.seqs ? decode_steps(a, b0 + lane) : 0;
+      const unsigned sum = wave_scan(mine);
+      if ((b ^ b0) < 64) {   // (b0 is a multiple of 64)
+        own = __builtin_amdgcn_readlane(mine, b - b0);
+        before = all + ((unsigned)__builtin_amdgcn_readlane((int)sum, b - b0) - (unsigned)own);
+      }
+      all += (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
+    }
+    const long per = deal_run(a, all), w0 = before / per;
+    at = (size_t)head * (a.deal + a.c.seqs) + w0 + b;
+    n = own ? (int)((before + own - 1) / per - w0) + 1 : 0;
+  }
   float mm = -INFINITY;
-  for (int i = lane; i < a.splits; i += 64) mm = fmaxf(mm, a.part_ml[2 * (at + i)]);
+  for (int i = lane; i < n; i += 64) mm = fmaxf(mm, a.part_ml[2 * (at + i)]);
   mm = wave_max(mm);
   float l = 0.0f, acc[E] = {};
-  for (int i0 = 0; i0 < a.splits; i0 += 64) {
+  for (int i0 = wave * 16; i0 < n; i0 += 64) {   // 16 parts at a time
     float w = 0.0f;
-    if (i0 + lane < a.splits) {
+    if (lane < 16 && i0 + lane < n) {
       const float2 x = *(const float2*)(a.part_ml + 2 * (at + i0 + lane));
       w = x.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x.x - mm);
       l += x.y * w;
     }
-    const int n = min(64, a.splits - i0);
-    for (int j0 = 0; j0 < n; j0 += 8) {
-      float x[8][E], wj[8];
+    float x[16][E];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        wj[j] = j0 + j < n ? __shfl(w, j0 + j, 64) : 0.0f;
-        const float* po = a.part_o + (at + min(i0 + j0 + j, a.splits - 1)) * D + lane * E;
+    for (int j = 0; j < 16; ++j) {
+      const float* po = a.part_o + (at + min(i0 + j, n - 1)) * D + lane * E;
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[j][e] = po[e];
-      }
+      for (int e = 0; e < E; ++e) x[j][e] = po[e];
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (wj[j] != 0.0f)
+    for (int j = 0; j < 16; ++j) {
+      const float wj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
+      if (wj != 0.0f)   // (a part without keys holds no sums)
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = fmaf(wj[j], x[j][e], acc[e]);
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(wj, x[j][e], acc[e]);
     }
   }
   l = group_sum<64>(l);
-  T* out = (T*)a.out + (size_t)m * a.ldo + (size_t)head * D + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = (T)(l == 0.0f ? 0.0f : acc[e] / l);
+  for (int e = 0; e < E; ++e) sums[wave][lane * E + e] = acc[e];
+  if (lane == 0) ls[wave] = l;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  const int d = threadIdx.x;
+  l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
+  const float o = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
+  ((T*)a.out)[(size_t)m * a.ldo + (size_t)head * D + d] = (T)(l == 0.0f ? 0.0f : o / l);
 }
 
 // A call's kernel and splits of its keys: enough workgroups for the CUs.
 struct PagedPlan {
   bool block;   // paged_prefill.hip
   long tiles;
-  int splits, steps, most;   // most: splits of any length
+  int splits, most;   // most: splits of any length
+  int deal;           // workgroups a kv-head and tile of query heads that share all keys (0: a workgroup a tile and split)
 };
 static PagedPlan paged_plan(const ti_paged_cache* c, const ti_paged_attn_args* p) {
   const int G = p->heads / c->kv_heads;
@@ -387,40 +512,45 @@ static PagedPlan paged_plan(const ti_paged_cache* c, const ti_paged_attn_args* p
   long span = (long)c->table_ld * c->page;
   if (p->max_len > 0) span = std::min<long>(span, p->max_len);
   if (p->window > 0 && !p->prefix) span = std::min<long>(span, (long)p->window + cols);
-  const long units = std::max(1l, tiles * c->kv_heads);
-  if (block) {
-    const long steps = (span + 63) / 64, most = std::max(1l, std::min(256 / units, 64l));
-    return {true, tiles, (int)std::max(1l, std::min(most, steps / 8)), 0, (int)most};
+  if (block) {   // (of the tiles that there can be, one a sequence may be empty)
+    const long full = std::max(1l, (columns + cols - 1) / cols * c->kv_heads), steps = (span + 63) / 64, most = std::max(1l, std::min(256 / full, 64l));
+    return {true, tiles, (int)std::max(1l, std::min(most, steps / 4)), (int)most, 0};
   }
-  const long steps = (span + kStreamKeys - 1) / kStreamKeys;
-  const long most = std::min((1024 + units - 1) / units, 256l);
-  const long splits = std::max(1l, std::min(most, (steps + kStreamWaves - 1) / kStreamWaves));
-  const int per = (int)(((steps + splits - 1) / splits + kStreamWaves - 1) / kStreamWaves * kStreamWaves);
-  return {false, tiles, (int)std::max(1l, (steps + per - 1) / per), per, (int)most};
+  const long units = std::max(1l, tiles * c->kv_heads);
+  if (!p->row_start) {
+    const int per_cu = c->kv_type == TI_KV_I8 && c->head_dim < 256 ? 2 : 1, deal = (int)std::max(1l, 256l * per_cu / (c->kv_heads * (long)((G + 15) / 16)));
+    return {false, tiles, 1, 1, span > 256 ? deal : 0};
+  }
+  const long steps = (span + kStreamKeys - 1) / kStreamKeys, most = std::min((1024 + units - 1) / units, 256l);
+  return {false, tiles, (int)std::max(1l, std::min(most, (steps + kStreamWaves - 1) / kStreamWaves)), (int)most, 0};
 }
 
 template <int D, class T>
 int launch_attn(PagedAttn a, const PagedPlan& plan, const ti_paged_cache* c, hipStream_t s) {
+  const bool i8 = c->kv_type == TI_KV_I8;
   if (plan.block) {
     if (const int rc = paged_block(a, c, plan.tiles, s)) return rc;
+  } else if (plan.deal) {
+    hipLaunchKernelGGL((i8 ? paged_deal_kernel<D, T, true> : paged_deal_kernel<D, T, false>), dim3(plan.deal, c->kv_heads * ((a.G + 15) / 16)),
+                       dim3(64 * kStreamWaves), 0, s, a);
+    TI_LAUNCH_CHECK("paged_deal_kernel");
   } else {
-    const dim3 grid((unsigned)plan.tiles, c->kv_heads, plan.splits);
-    if (c->kv_type == TI_KV_I8)
-      hipLaunchKernelGGL((paged_stream_kernel<D, T, true>), grid, dim3(64 * kStreamWaves), 0, s, a);
-    else
-      hipLaunchKernelGGL((paged_stream_kernel<D, T, false>), grid, dim3(64 * kStreamWaves), 0, s, a);
+    hipLaunchKernelGGL((i8 ? paged_stream_kernel<D, T, true> : paged_stream_kernel<D, T, false>), dim3((unsigned)plan.tiles, c->kv_heads, plan.splits),
+                       dim3(64 * kStreamWaves), 0, s, a);
     TI_LAUNCH_CHECK("paged_stream_kernel");
   }
-  if (plan.splits > 1) {
-    hipLaunchKernelGGL((paged_join_kernel<D, T>), dim3(a.r.rows, (a.heads + 3) / 4), dim3(256), 0, s, a);
+  if (a.part_o) {
+    hipLaunchKernelGGL((paged_join_kernel<D, T>), dim3(a.r.rows, a.heads), dim3(256), 0, s, a);
     TI_LAUNCH_CHECK("paged_join_kernel");
   }
   return TI_OK;
 }
 
-static size_t part_bytes(const ti_paged_cache* c, const ti_paged_attn_args* p, int splits) {
-  return splits < 2 ? 0 : (size_t)p->rows * p->heads * splits * ((size_t)c->head_dim + 2) * sizeof(float);
+// Parts of all rows and heads.
+static size_t parts(const ti_paged_cache* c, const ti_paged_attn_args* p, const PagedPlan& plan, int splits) {
+  return plan.deal ? (size_t)p->heads * (plan.deal + c->seqs) : splits > 1 ? (size_t)p->rows * p->heads * splits : 0;
 }
+static size_t part_bytes(const ti_paged_cache* c, size_t n) { return n * ((size_t)c->head_dim + 2) * sizeof(float); }
 
 static int check_attn(const ti_paged_cache* c, const ti_paged_attn_args* p, const char* who) {
   if (const int rc = ti_paged_check(c, who)) return rc;
@@ -445,14 +575,13 @@ static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_strea
     return ti_set_error(TI_ERR_ARG, "%s: pointers are not aligned", who);
   if (p->rows == 0) return TI_OK;
   const PagedPlan plan = paged_plan(c, p);
-  const size_t need = part_bytes(c, p, plan.splits);
+  const size_t n = parts(c, p, plan, plan.splits), need = part_bytes(c, n);
   if (need && (!p->workspace || p->workspace_bytes < (int64_t)need))
     return ti_set_error(TI_ERR_ARG, "%s: workspace of %ld bytes, %zu needed", who, (long)(p->workspace ? p->workspace_bytes : 0), need);
-  const size_t n_o = (size_t)p->rows * p->heads * plan.splits * c->head_dim;
   float* ws = (float*)p->workspace;
   const float cap = p->softcap;
-  const PagedAttn a = {ti_paged_form(c), {p->row_start, p->rows}, p->q, p->out, p->slopes, p->first, p->prefix, ws, need ? ws + n_o : nullptr,
-                       p->heads, p->heads / c->kv_heads, p->ldq, p->ldo, p->window, plan.splits, plan.steps,
+  const PagedAttn a = {ti_paged_form(c), {p->row_start, p->rows}, p->q, p->out, p->slopes, p->first, p->prefix, n ? ws : nullptr,
+                       n ? ws + n * c->head_dim : nullptr, p->heads, p->heads / c->kv_heads, p->ldq, p->ldo, p->window, plan.splits, plan.deal,
                        cap > 0.0f ? 2.0f * p->scale * kPagedLog2e / cap : p->scale * kPagedLog2e, cap * kPagedLog2e};
   return TI_PAGED_FORM(c, launch_attn, a, plan, c, (hipStream_t)stream_);
 }
@@ -461,7 +590,10 @@ static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_strea
 
 extern "C" size_t ti_paged_workspace_bytes(const ti_paged_cache* c, const ti_paged_attn_args* a) {
   if (ti::check_attn(c, a, "ti_paged_workspace_bytes")) return 0;
-  return ti::part_bytes(c, a, ti::paged_plan(c, a).most);
+  ti_paged_attn_args any = *a;   // (of any length)
+  any.max_len = any.window = 0;
+  const ti::PagedPlan plan = ti::paged_plan(c, &any);
+  return ti::part_bytes(c, ti::parts(c, a, plan, plan.most));
 }
 
 extern "C" int ti_paged_decode(const ti_paged_cache* c, const ti_paged_attn_args* a, ti_stream_t s) {

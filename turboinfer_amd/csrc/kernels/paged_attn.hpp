@@ -16,10 +16,10 @@ struct PagedAttn {
   const float* slopes;
   const int32_t* first;
   const int32_t* prefix;
-  float* part_o;    // splits > 1: [row][head][split][D] relative to 2^part_ml[..][0]
-  float* part_ml;   // [row][head][split][2]
-  int heads, G, ldq, ldo, window, splits, steps;   // steps: of keys, of a split at a time
-  float f, cap;     // weights are 2^(f s), or with a cap 2^(cap tanh(s ..)): paged_score
+  float* part_o;    // sums of parts of the keys (NULL: none), relative to 2^part_ml[..][0]: [row][head][split][D]; dealt: [head][deal + seqs][D]
+  float* part_ml;   // [..][2]: reference, denominator
+  int heads, G, ldq, ldo, window, splits, deal;
+  float f, cap;     // weights are 2^(f s), or with a cap paged_capped's
 };
 
 constexpr float kPagedLog2e = 1.44269504088896341f;
@@ -44,10 +44,9 @@ __device__ __forceinline__ uint32_t i8_of(uint32_t x) {
   return i8_pair(__builtin_amdgcn_perm(0u, x, HI ? 0x0c030c02u : 0x0c010c00u));
 }
 
-// Score s = q . k (int8: in the scale's units) as an exponent of 2.  With a cap: cap (1 - 2 / (e^(2 s / c) + 1)), f holding 2 scale
-// log2 e / c and cap c log2 e; its error is 2^-23 cap.
-__device__ __forceinline__ float paged_score(float s, float f, float cap) {
-  if (cap == 0.0f) return s * f;
+// A score s = q . k (int8: in the scale's units) under a cap c, as an exponent of 2: cap (1 - 2 / (e^(2 s scale / c) + 1)), f holding
+// 2 scale log2 e / c and cap c log2 e; its error is 2^-22 cap.
+__device__ __forceinline__ float paged_capped(float s, float f, float cap) {
   return fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * f) + 1.0f), cap);
 }
 

@@ -20,7 +20,7 @@ struct AppendArgs {
   void* q;
   const float* rope;
   int heads, ldx, ldq, rope_len, rot_dim, halves;
-  int row_parts;   // blocks of y that take rows; the others take int8 blocks (2 a kv-head)
+  int row_parts, chunks;   // workgroups of a row, 8-dimension chunks that it has (the other workgroups take int8 blocks, 2 a kv-head)
 };
 
 template <class X>
@@ -40,30 +40,38 @@ __device__ __forceinline__ void load8(const X* x, float* v) {
   }
 }
 
-// Dimensions d .. d + 7 of a head at x, rotated by cs (this position's [rot_dim / 2] pairs; NULL: as they are).
+// Dimensions d .. d + 7 of a head at x and those that they are rotated with (rot_dim 0: not rotated), and their rotation by cs (this
+// position's [rot_dim / 2] pairs).
+struct Dims8 {
+  float v[8], o[8];
+};
 template <class X>
-__device__ __forceinline__ void rotated8(const X* x, int d, const float* cs, int rot_dim, int halves, float* v) {
-  load8(x + d, v);
-  if (!cs || d >= rot_dim) return;
+__device__ __forceinline__ Dims8 dims8(const X* x, int d, int rot_dim, int halves) {
+  Dims8 r;
+  load8(x + d, r.v);
+  if (halves && d < rot_dim) load8(x + (d < rot_dim >> 1 ? d + (rot_dim >> 1) : d - (rot_dim >> 1)), r.o);
+  return r;
+}
+__device__ __forceinline__ void rotate8(Dims8& r, int d, const float* cs, int rot_dim, int halves) {
+  if (d >= rot_dim) return;
   if (!halves) {
     float t[8];
     load8(cs + d, t);
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const float a = v[e], b = v[e + 1];
-      v[e] = a * t[e] - b * t[e + 1];
-      v[e + 1] = a * t[e + 1] + b * t[e];
+      const float a = r.v[e], b = r.v[e + 1];
+      r.v[e] = a * t[e] - b * t[e + 1];
+      r.v[e + 1] = a * t[e + 1] + b * t[e];
     }
     return;
   }
   const int half = rot_dim >> 1, i = d < half ? d : d - half;
-  float o[8], t[16];
-  load8(x + (d < half ? d + half : d - half), o);
+  float t[16];
   load8(cs + 2 * i, t);
   load8(cs + 2 * i + 8, t + 8);
   const float sign = d < half ? -1.0f : 1.0f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = v[e] * t[2 * e] + sign * (o[e] * t[2 * e + 1]);
+  for (int e = 0; e < 8; ++e) r.v[e] = r.v[e] * t[2 * e] + sign * (r.o[e] * t[2 * e + 1]);
 }
 
 // One int8 block of a kv-head: D * 2 threads, 8 dimensions of a token each.
@@ -89,11 +97,13 @@ __device__ void append_block(const AppendArgs& a, int slot, int part, float* red
   const float s_old = has_old ? *scale : 0.0f;
   uint2 q = {0, 0};
   if (old) q = *(const uint2*)cell;
-  float v[8] = {};
+  Dims8 y = {};
   if (fresh) {
-    const X* x = (const X*)a.x + (size_t)(s.row0 + (pos - s.pos0)) * a.ldx + (size_t)(a.heads + kvh + (is_v ? a.c.s.kv_heads : 0)) * D;
-    rotated8(x, d, is_v || !a.rope ? nullptr : a.rope + (size_t)pos * a.rot_dim, a.rot_dim, a.halves, v);
+    const int rot = is_v ? 0 : a.rot_dim;
+    y = dims8((const X*)a.x + (size_t)(s.row0 + (pos - s.pos0)) * a.ldx + (size_t)(a.heads + kvh + (is_v ? a.c.s.kv_heads : 0)) * D, d, rot, a.halves);
+    rotate8(y, d, a.rope + (size_t)pos * a.rot_dim, rot, a.halves);
   }
+  const float* v = y.v;
   // the largest magnitude by its bits: infinities and NaN are above every number
   uint32_t most = 0;
 #pragma unroll
@@ -132,35 +142,41 @@ __device__ void append_block(const AppendArgs& a, int slot, int part, float* red
   }
 }
 
-// Rows: q, and k and v of 16-bit caches.  Grid (rows or int8 blocks, parts); D * 2 threads.
+// Rows: q, and k and v of 16-bit caches.  D * 2 threads; a row's workgroups, then the int8 blocks'.
 template <int D, class T, class X, bool I8>
 __global__ __launch_bounds__(2 * D) void paged_append_kernel(const AppendArgs a) {
   constexpr int CH = D / 8;
   __shared__ float red[D / 32];
-  if (I8 && (int)blockIdx.y >= a.row_parts) {
-    append_block<D, X>(a, blockIdx.x, blockIdx.y - a.row_parts, red);
+  const int row_groups = a.r.rows * a.row_parts;
+  if (I8 && (int)blockIdx.x >= row_groups) {
+    const int i = blockIdx.x - row_groups, n = 2 * a.c.s.kv_heads;
+    append_block<D, X>(a, i / n, i % n, red);
     return;
   }
-  const int m = blockIdx.x, at = blockIdx.y * 2 * D + threadIdx.x, head = at / CH, d = at % CH * 8;
-  if (m >= a.r.rows) return;
+  const int m = blockIdx.x / a.row_parts, stride = a.row_parts * 2 * D;
+  int at = (blockIdx.x - m * a.row_parts) * 2 * D + threadIdx.x;
+  const X* x = (const X*)a.x + (size_t)m * a.ldx;
+  // (the first values are asked for before it is known where they go)
+  auto fetch = [&] { return dims8(x + at / CH * D, at % CH * 8, at / CH < a.heads + a.c.s.kv_heads ? a.rot_dim : 0, a.halves); };
+  Dims8 y = {};
+  if (at < a.chunks) y = fetch();
   const int b = a.r.start ? paged_find(a.c.seqs, m, [&](int j) { return (long)a.r.start[j]; }) : m;
-  if (b >= a.c.seqs) return;
   const PagedSeq s = paged_seq(a.c, a.r, b);
   const int pos = s.pos0 + (m - s.row0);
   if (m < s.row0 || m >= s.row0 + s.n || pos < 0 || pos >= a.c.s.blocks * kPagedBlock || (a.rope && pos >= a.rope_len)) return;
-  const int n_heads = a.heads + (I8 ? 0 : 2 * a.c.s.kv_heads);
-  if (head >= n_heads) return;
-  float v[8];
-  const bool is_v = head >= a.heads + a.c.s.kv_heads;
-  rotated8((const X*)a.x + (size_t)m * a.ldx + (size_t)head * D, d, is_v || !a.rope ? nullptr : a.rope + (size_t)pos * a.rot_dim, a.rot_dim, a.halves, v);
-  if (head < a.heads) {
-    *(u16x8*)((T*)a.q + (size_t)m * a.ldq + head * D + d) = pack8<T>(v);
-    return;
+  const int blk = pos / kPagedBlock, entry = I8 ? 0 : a.c.table[(size_t)b * a.c.table_ld + paged_column(a.c.s, blk)];
+  for (; at < a.chunks; at += stride) {
+    const int head = at / CH, d = at % CH * 8;
+    const bool is_v = head >= a.heads + a.c.s.kv_heads;
+    if (at >= stride) y = fetch();
+    rotate8(y, d, a.rope + (size_t)pos * a.rot_dim, is_v ? 0 : a.rot_dim, a.halves);
+    if (I8 || head < a.heads) {
+      *(u16x8*)((T*)a.q + (size_t)m * a.ldq + head * D + d) = pack8<T>(y.v);
+    } else {
+      const int kvh = head - a.heads - (is_v ? a.c.s.kv_heads : 0), id = paged_block(a.c.s, entry, kvh, blk);
+      if (id >= 0) *(u16x8*)((T*)(is_v ? a.c.v : a.c.k) + (size_t)id * (kPagedBlock * D) + (pos % kPagedBlock) * D + d) = pack8<T>(y.v);
+    }
   }
-  const int kvh = head - a.heads - (is_v ? a.c.s.kv_heads : 0), blk = pos / kPagedBlock;
-  const int id = paged_block(a.c.s, a.c.table[(size_t)b * a.c.table_ld + paged_column(a.c.s, blk)], kvh, blk);
-  if (id < 0) return;
-  *(u16x8*)((T*)(is_v ? a.c.v : a.c.k) + (size_t)id * (kPagedBlock * D) + (pos % kPagedBlock) * D + d) = pack8<T>(v);
 }
 
 struct ReadArgs {
@@ -205,13 +221,17 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const ReadArgs a) {
 template <int D, class T>
 int append(AppendArgs a, const ti_paged_cache* c, int x_f32, hipStream_t s) {
   const bool i8 = c->kv_type == TI_KV_I8;
-  const int chunks = (a.heads + (i8 ? 0 : 2 * c->kv_heads)) * (D / 8);
-  a.row_parts = (chunks + 2 * D - 1) / (2 * D);
+  a.chunks = (a.heads + (i8 ? 0 : 2 * c->kv_heads)) * (D / 8);
+  // few rows: a chunk a thread; many: a row a workgroup, which looks its place up once.  us, 32 heads on 8 of 128: 32 rows 6.7 / 7.2, 512 6.4 /
+  // 7.0, 2048 12.3 / 11.0, 8000 50.6 / 42.8 (4.7 TB/s, as a large copy)
+  a.row_parts = (a.chunks + 2 * D - 1) / (2 * D);
+  if (a.r.rows >= 1024 && a.row_parts > 1) a.row_parts = 1;
   const long slots = !i8 ? 0 : a.r.start ? paged_touches(a.r.rows, c->seqs) : a.r.rows;
-  const dim3 grid((unsigned)std::max<long>(a.row_parts ? a.r.rows : 0, slots), a.row_parts + (i8 ? 2 * c->kv_heads : 0));
+  const long grid = (long)a.r.rows * a.row_parts + slots * 2 * c->kv_heads;
+  if (grid > INT32_MAX) return ti_set_error(TI_ERR_ARG, "ti_paged_append: %d rows of %d heads in a call", a.r.rows, a.heads + 2 * c->kv_heads);
   auto* fn = i8 ? (x_f32 ? paged_append_kernel<D, T, float, true> : paged_append_kernel<D, T, T, true>)
                 : (x_f32 ? paged_append_kernel<D, T, float, false> : paged_append_kernel<D, T, T, false>);
-  hipLaunchKernelGGL(fn, grid, dim3(2 * D), 0, s, a);
+  hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(2 * D), 0, s, a);
   TI_LAUNCH_CHECK("paged_append_kernel");
   return TI_OK;
 }
@@ -280,8 +300,8 @@ extern "C" int ti_paged_append(const ti_paged_cache* c, const ti_paged_append_ar
   if (p->rope_cs && (p->rot_dim < 16 || p->rot_dim > D || p->rot_dim % 16 || p->rope_len < 1 || (p->rope_kind != TI_ROPE_PAIRS && p->rope_kind != TI_ROPE_HALVES)))
     return ti_set_error(TI_ERR_ARG, "ti_paged_append: rotation of %d dimensions, %d positions, kind %d", p->rot_dim, p->rope_len, p->rope_kind);
   if (p->rows == 0) return TI_OK;
-  const ti::AppendArgs a = {ti_paged_form(c), {p->row_start, p->rows}, p->x, p->q, p->rope_cs, p->heads, p->ldx, p->ldq, p->rope_len, p->rot_dim,
-                            p->rope_kind == TI_ROPE_HALVES, 0};
+  const ti::AppendArgs a = {ti_paged_form(c), {p->row_start, p->rows}, p->x, p->q, p->rope_cs, p->heads, p->ldx, p->ldq, p->rope_len,
+                            p->rope_cs ? p->rot_dim : 0, p->rope_kind == TI_ROPE_HALVES, 0, 0};
   using namespace ti;
   return TI_PAGED_FORM(c, ti::append, a, c, p->x_f32, (hipStream_t)stream);
 }

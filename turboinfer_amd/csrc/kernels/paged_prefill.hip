@@ -146,7 +146,7 @@ __global__ __launch_bounds__(BlockForm<D>::NT, D == 256 ? 1 : 2) void paged_bloc
       if (to >= 0) {
         k = a.c.ks[to];
         v = a.c.vs[to];
-        v = v < kPagedTiny ? kPagedTiny : v;
+        v = v < kPagedTiny ? kPagedTiny : v;   // (a user's 0)
       }
     }
   };
@@ -261,19 +261,38 @@ __global__ __launch_bounds__(BlockForm<D>::NT, D == 256 ? 1 : 2) void paged_bloc
         }
       }
     }
-    const bool plain = !I8 && a.cap == 0.0f && !a.slopes && f > 0.0f;
-    float mx = -INFINITY;
-    if (!plain) {
-      const float base = (float)(key0 + 4 * h - p);
+    // exponents of 2: mul[block] s + add[block], or s itself where a cap or a slope makes them
+    float mul[4], add[4], mx = -INFINITY;
+    if (a.cap != 0.0f || a.slopes) {
+      if (a.cap != 0.0f) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[t][i] = paged_capped(sc[t][i], fk[2 * t + (i >> 3)], a.cap);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) fk[t] = 1.0f;
+      }
+      const float base = slope * (float)(key0 + 4 * h - p);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float v = paged_score(sc[t][i], fk[2 * t + (i >> 3)], a.cap);
-          if (a.slopes) v = fmaf(slope, base + (float)(32 * t + 8 * (i >> 2) + (i & 3)), v);
-          if constexpr (I8) v += vl[2 * t + (i >> 3)];
-          sc[t][i] = v;
+          float more = fmaf(slope, (float)(32 * t + 8 * (i >> 2) + (i & 3)), base);
+          if constexpr (I8) more += vl[2 * t + (i >> 3)];
+          sc[t][i] = fmaf(sc[t][i], fk[2 * t + (i >> 3)], more);
         }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        mul[t] = 1.0f;
+        add[t] = 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {   // (what is masked stays -inf: a factor > 0, and none of a block that is not seen)
+        const bool none = I8 && ragged && !(see[t >> 1] >> 8 * (t & 1) & 255);
+        mul[t] = none ? 1.0f : fk[t] < 0x1p-120f ? 0x1p-120f : fk[t];
+        add[t] = none ? 0.0f : vl[t];
+      }
     }
     if (ragged) {
 #pragma unroll
@@ -283,11 +302,14 @@ __global__ __launch_bounds__(BlockForm<D>::NT, D == 256 ? 1 : 2) void paged_bloc
           if (!(see[t] >> i & 1)) sc[t][i] = -INFINITY;
     }
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 4; ++t) {
+      float x = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[t][i]);
-    const float mul = plain ? f : 1.0f;
-    mx = xor32_max(mx) * mul;
+      for (int e = 0; e < 8; ++e) x = fmaxf(x, sc[t >> 1][8 * (t & 1) + e]);
+      mx = fmaxf(mx, I8 ? fmaf(x, mul[t], add[t]) : x);
+    }
+    mx = xor32_max(mx);
+    if constexpr (!I8) mx *= mul[0];
     if (__builtin_amdgcn_ballot_w64(mx > mr + 15.0f) != 0) {
       const float mn = mx > mr + 15.0f ? mx - 7.0f : mr, alpha = mn == mr ? 1.0f : __builtin_amdgcn_exp2f(mr - mn);
       mr = mn;
@@ -302,9 +324,10 @@ __global__ __launch_bounds__(BlockForm<D>::NT, D == 256 ? 1 : 2) void paged_bloc
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float l = 0.0f;
+        const float m1 = mul[2 * t + u], a1 = add[2 * t + u] - off;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-          const float w0 = __builtin_amdgcn_exp2f(fmaf(sc[t][8 * u + e], mul, -off)), w1 = __builtin_amdgcn_exp2f(fmaf(sc[t][8 * u + e + 1], mul, -off));
+          const float w0 = __builtin_amdgcn_exp2f(fmaf(sc[t][8 * u + e], m1, a1)), w1 = __builtin_amdgcn_exp2f(fmaf(sc[t][8 * u + e + 1], m1, a1));
           l += w0 + w1;
           typedef M M2 __attribute__((ext_vector_type(2)));
           const M2 w = __builtin_convertvector((f32x2){w0, w1}, M2);

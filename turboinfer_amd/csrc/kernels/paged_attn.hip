@@ -206,11 +206,10 @@ __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_
             vi[t] = ragged && !(see >> 4 * t & 15) ? 0.0f : __builtin_amdgcn_rcpf(sv);   // (0 of a block, whose scale may be NaN)
           }
           if (a.cap != 0.0f) {
-            float cap = a.cap;
-            asm volatile("" : "+s"(cap));
+            asm volatile("" : "+v"(ft));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[t][e] = paged_capped(sc[t][e], ft, cap);
-            ft = 1.0f;
+            for (int e = 0; e < 4; ++e) sc[t][e] = paged_capped(sc[t][e], ft);
+            ft = a.cap;
           }
           if (a.slopes) {
             float slope_ = slope;
@@ -430,34 +429,28 @@ __global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_dea
   }
 }
 
-// A workgroup a (row, head): its parts joined, four waves in turn.
+// The parts of single tokens: a workgroup a (row, head), four waves in turn.
 template <int D, class T>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn a) {
+__global__ __launch_bounds__(256) void deal_join_kernel(const PagedAttn a) {
   constexpr int E = D / 64;
   __shared__ float sums[4][D], ls[4];
   const int lane = threadIdx.x & 63, m = blockIdx.x, head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = a.r.start ? paged_find(a.c.seqs, m, [&](int j) { return (long)a.r.start[j]; }) : m;
-  const PagedSeq s = paged_seq(a.c, a.r, b);
-  const int p = s.pos0 + (m - s.row0);
-  if (m < s.row0 || m >= s.row0 + s.n || p < 0 || p >= a.c.s.blocks * kPagedBlock) return;
-  size_t at = ((size_t)m * a.heads + head) * a.splits;
-  int n = a.splits;
-  if (a.deal) {
-    long all = 0, before = 0;   // steps of all sequences, of those in front of b
-    int own = 0;
-    for (int b0 = 0; b0 < a.c.seqs; b0 += 64) {
-      const int mine = b0 + lane < a.c.seqs ? decode_steps(a, b0 + lane) : 0;
-      const unsigned sum = wave_scan(mine);
-      if ((b ^ b0) < 64) {   // (b0 is a multiple of 64)
-        own = __builtin_amdgcn_readlane(mine, b - b0);
-        before = all + ((unsigned)__builtin_amdgcn_readlane((int)sum, b - b0) - (unsigned)own);
-      }
-      all += (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
+  const int b = m, p = a.c.len[b] - 1;
+  if (p < 0 || p >= a.c.s.blocks * kPagedBlock) return;
+  long all = 0, before = 0;   // steps of all sequences, of those in front of b
+  int own = 0;
+  for (int b0 = 0; b0 < a.c.seqs; b0 += 64) {
+    const int mine = b0 + lane < a.c.seqs ? decode_steps(a, b0 + lane) : 0;
+    const unsigned sum = wave_scan(mine);
+    if ((b ^ b0) < 64) {   // (b0 is a multiple of 64)
+      own = __builtin_amdgcn_readlane(mine, b - b0);
+      before = all + ((unsigned)__builtin_amdgcn_readlane((int)sum, b - b0) - (unsigned)own);
     }
-    const long per = deal_run(a, all), w0 = before / per;
-    at = (size_t)head * (a.deal + a.c.seqs) + w0 + b;
-    n = own ? (int)((before + own - 1) / per - w0) + 1 : 0;
+    all += (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
   }
+  const long per = deal_run(a, all), w0 = before / per;
+  const size_t at = (size_t)head * (a.deal + a.c.seqs) + w0 + b;
+  const int n = own ? (int)((before + own - 1) / per - w0) + 1 : 0;
   float mm = -INFINITY;
   for (int i = lane; i < n; i += 64) mm = fmaxf(mm, a.part_ml[2 * (at + i)]);
   mm = wave_max(mm);
@@ -496,40 +489,101 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn a) {
   ((T*)a.out)[(size_t)m * a.ldo + (size_t)head * D + d] = (T)(l == 0.0f ? 0.0f : o / l);
 }
 
+// The splits of rows: D / 4 threads a (row, head), 1024 / D heads a workgroup.  Grid (rows, groups of heads).
+template <int D, class T>
+__global__ __launch_bounds__(256) void split_join_kernel(const PagedAttn a) {
+  constexpr int NT = D / 4, NH = 256 / NT, U = 8;
+  const int m = blockIdx.x, d = threadIdx.x % NT * 4, head = blockIdx.y * NH + threadIdx.x / NT;
+  const int b = a.r.start ? paged_find(a.c.seqs, m, [&](int j) { return (long)a.r.start[j]; }) : m;
+  const PagedSeq s = paged_seq(a.c, a.r, b);
+  const int p = s.pos0 + (m - s.row0);
+  if (m < s.row0 || m >= s.row0 + s.n || p < 0 || p >= a.c.s.blocks * kPagedBlock || head >= a.heads) return;
+  const size_t at = ((size_t)m * a.heads + head) * a.splits;
+  const float2* ml = (const float2*)a.part_ml + at;
+  const float* po = a.part_o + at * D + d;
+  float mm = -INFINITY, l = 0.0f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < a.splits; i0 += U) {   // (the sums so far follow the reference)
+    float2 x[U];
+    f32x4 y[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) x[i] = i0 + i < a.splits ? ml[i0 + i] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+    for (int i = 0; i < U; ++i) y[i] = *(const f32x4*)(po + (size_t)min(i0 + i, a.splits - 1) * D);
+    float mn = mm;
+#pragma unroll
+    for (int i = 0; i < U; ++i) mn = fmaxf(mn, x[i].x);
+    const float back = mm == mn ? 1.0f : __builtin_amdgcn_exp2f(mm - mn);
+    mm = mn;
+    l *= back;
+    acc *= back;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const float w = x[i].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x[i].x - mm);   // (a split without keys holds no sums)
+      l = fmaf(x[i].y, w, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = w != 0.0f ? fmaf(w, y[i][e], acc[e]) : acc[e];
+    }
+  }
+  typedef T Q4 __attribute__((ext_vector_type(4)));
+  Q4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = (T)(l == 0.0f ? 0.0f : acc[e] / l);
+  *(Q4*)((T*)a.out + (size_t)m * a.ldo + (size_t)head * D + d) = y;
+}
+
 // A call's kernel and splits of its keys: enough workgroups for the CUs.
 struct PagedPlan {
-  bool block;   // paged_prefill.hip
+  int waves;          // of paged_prefill.hip's kernel (0: this file's)
   long tiles;
   int splits, most;   // most: splits of any length
   int deal;           // workgroups a kv-head and tile of query heads that share all keys (0: a workgroup a tile and split)
+  long filled;        // workgroups with work, about
 };
 static PagedPlan paged_plan(const ti_paged_cache* c, const ti_paged_attn_args* p) {
   const int G = p->heads / c->kv_heads;
   const long columns = (long)p->rows * G;
-  const bool block = p->row_start && columns >= 64l * c->seqs;
-  const int cols = block ? paged_block_cols(c->head_dim) : 16;
-  const long tiles = p->row_start ? paged_tiles(columns, c->seqs, cols) : (long)c->seqs * ((G + 15) / 16);
   long span = (long)c->table_ld * c->page;
   if (p->max_len > 0) span = std::min<long>(span, p->max_len);
-  if (p->window > 0 && !p->prefix) span = std::min<long>(span, (long)p->window + cols);
-  if (block) {   // (of the tiles that there can be, one a sequence may be empty)
-    const long full = std::max(1l, (columns + cols - 1) / cols * c->kv_heads), steps = (span + 63) / 64, most = std::max(1l, std::min(256 / full, 64l));
-    return {true, tiles, (int)std::max(1l, std::min(most, steps / 4)), (int)most, 0};
+  const long per_seq = columns / c->seqs;
+  // From 32 columns a sequence on keys are shared in LDS.  us, stream / block: 16 sequences behind 2k, 8 rows of 32 heads on 8 55 / 40, 16 rows 94 / 46;
+  // 8 behind 1k, 32 rows of 32 on 32 59 / 43; 32 behind 2k, 4 rows (16 columns) 70 / 70.
+  if (p->row_start && per_seq >= 32) {
+    // waves of a workgroup, workgroups that fill the CUs, least steps of a split
+    auto form = [&](int waves, long want, long least) {
+      const int cols = 32 * waves;
+      const long full = (long)c->seqs * ((per_seq + cols - 1) / cols) * c->kv_heads;
+      const long keys = p->window > 0 && !p->prefix ? std::min<long>(span, (long)p->window + cols) : span;
+      const long most = std::max(1l, std::min(want / full, 64l)), splits = std::max(1l, std::min(most, (keys + 63) / 64 / least));
+      return PagedPlan{waves, paged_tiles(columns, c->seqs, cols), (int)splits, (int)most, 0, full * splits};
+    };
+    if (c->head_dim == 256) return form(4, 256, 4);
+    // Eight waves read each block of keys from L2 and convert it once for twice the columns, two workgroups of four hide each other's
+    // waits: eight for long keys and enough columns, four where prompts are short, CUs would idle, or (heads of 64 in 16 bits) three
+    // workgroups of four fit a CU.  us, 8 / 4 waves, 32 heads on 8 of 128: 4000 rows 164 / 186, capped 205 / 242, 2 x 512 behind 7.5k in int8 194
+    // / 216, 128 behind 32k int8 108 / 126, 256 behind 8k 57 / 62; 1000 rows 38.6 / 37.8, 12 prompts of 40 - 640 60 / 54, 8 x 200 rows of 32 heads on
+    // 32 41 / 24, 64 x 64 rows 54 / 39; 512 rows 31 / 25 (64 workgroups of eight); heads of 64, 4000 rows 111 / 103, int8 130 / 149.
+    const PagedPlan wide = form(8, 256, 4);
+    return !(c->head_dim == 64 && c->kv_type == TI_KV_SAME) && per_seq >= 192 && span >= 2048 && wide.filled >= 192 ? wide : form(4, 512, 8);
   }
+  if (p->window > 0 && !p->prefix) span = std::min<long>(span, (long)p->window + 16);
+  const long tiles = p->row_start ? paged_tiles(columns, c->seqs, 16) : (long)c->seqs * ((G + 15) / 16);
   const long units = std::max(1l, tiles * c->kv_heads);
   if (!p->row_start) {
+    // 256 keys are a step or two of each wave: one launch.  Workgroups a CU: 1 (32 streams of 4k - 8k, f16 of 128 dims, 1 / 2 / 3: 146 / 151 / 151 us;
+    // 48 capped of 256 dims 87 / 100 / 122), but 2 of int8 heads up to 128 dims, whose waves convert (64 of 64 dims 60 / 50 / 52, 64 x 700 37 / 32 / 39).
     const int per_cu = c->kv_type == TI_KV_I8 && c->head_dim < 256 ? 2 : 1, deal = (int)std::max(1l, 256l * per_cu / (c->kv_heads * (long)((G + 15) / 16)));
-    return {false, tiles, 1, 1, span > 256 ? deal : 0};
+    return {0, tiles, 1, 1, span > 256 ? deal : 0, 0};
   }
   const long steps = (span + kStreamKeys - 1) / kStreamKeys, most = std::min((1024 + units - 1) / units, 256l);
-  return {false, tiles, (int)std::max(1l, std::min(most, (steps + kStreamWaves - 1) / kStreamWaves)), (int)most, 0};
+  return {0, tiles, (int)std::max(1l, std::min(most, (steps + kStreamWaves - 1) / kStreamWaves)), (int)most, 0, 0};
 }
 
 template <int D, class T>
 int launch_attn(PagedAttn a, const PagedPlan& plan, const ti_paged_cache* c, hipStream_t s) {
   const bool i8 = c->kv_type == TI_KV_I8;
-  if (plan.block) {
-    if (const int rc = paged_block(a, c, plan.tiles, s)) return rc;
+  if (plan.waves) {
+    if (const int rc = paged_block_run(a, c, plan.waves, plan.tiles, s)) return rc;
   } else if (plan.deal) {
     hipLaunchKernelGGL((i8 ? paged_deal_kernel<D, T, true> : paged_deal_kernel<D, T, false>), dim3(plan.deal, c->kv_heads * ((a.G + 15) / 16)),
                        dim3(64 * kStreamWaves), 0, s, a);
@@ -540,8 +594,12 @@ int launch_attn(PagedAttn a, const PagedPlan& plan, const ti_paged_cache* c, hip
     TI_LAUNCH_CHECK("paged_stream_kernel");
   }
   if (a.part_o) {
-    hipLaunchKernelGGL((paged_join_kernel<D, T>), dim3(a.r.rows, a.heads), dim3(256), 0, s, a);
-    TI_LAUNCH_CHECK("paged_join_kernel");
+    constexpr int NH = 1024 / D;
+    if (a.deal)
+      hipLaunchKernelGGL((deal_join_kernel<D, T>), dim3(a.r.rows, a.heads), dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((split_join_kernel<D, T>), dim3(a.r.rows, (a.heads + NH - 1) / NH), dim3(256), 0, s, a);
+    TI_LAUNCH_CHECK("join kernel");
   }
   return TI_OK;
 }
@@ -582,7 +640,7 @@ static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_strea
   const float cap = p->softcap;
   const PagedAttn a = {ti_paged_form(c), {p->row_start, p->rows}, p->q, p->out, p->slopes, p->first, p->prefix, n ? ws : nullptr,
                        n ? ws + n * c->head_dim : nullptr, p->heads, p->heads / c->kv_heads, p->ldq, p->ldo, p->window, plan.splits, plan.deal,
-                       cap > 0.0f ? 2.0f * p->scale * kPagedLog2e / cap : p->scale * kPagedLog2e, cap * kPagedLog2e};
+                       cap > 0.0f ? 2.0f * p->scale * kPagedLog2e / cap : p->scale * kPagedLog2e, 2.0f * cap * kPagedLog2e};
   return TI_PAGED_FORM(c, launch_attn, a, plan, c, (hipStream_t)stream_);
 }
 

@@ -19,7 +19,7 @@ struct PagedAttn {
   float* part_o;    // sums of parts of the keys (NULL: none), relative to 2^part_ml[..][0]: [row][head][split][D]; dealt: [head][deal + seqs][D]
   float* part_ml;   // [..][2]: reference, denominator
   int heads, G, ldq, ldo, window, splits, deal;
-  float f, cap;     // weights are 2^(f s), or with a cap paged_capped's
+  float f, cap;     // weights are 2^(f s), or with a cap 2^(cap paged_capped(s, f))
 };
 
 constexpr float kPagedLog2e = 1.44269504088896341f;
@@ -44,11 +44,9 @@ __device__ __forceinline__ uint32_t i8_of(uint32_t x) {
   return i8_pair(__builtin_amdgcn_perm(0u, x, HI ? 0x0c030c02u : 0x0c010c00u));
 }
 
-// A score s = q . k (int8: in the scale's units) under a cap c, as an exponent of 2: cap (1 - 2 / (e^(2 s scale / c) + 1)), f holding
-// 2 scale log2 e / c and cap c log2 e; its error is 2^-22 cap.
-__device__ __forceinline__ float paged_capped(float s, float f, float cap) {
-  return fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * f) + 1.0f), cap);
-}
+// A score under a cap c, c tanh(x) = c - 2 c / (e^2x + 1): what 2 c log2 e (PagedAttn::cap) is multiplied with to an exponent of 2, without the
+// first term, which all keys have.  f: 2 scale log2 e / c (int8: times the keys' scale).
+__device__ __forceinline__ float paged_capped(float s, float f) { return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s * f)); }
 
 // Keys that a row at token p sees: [lo, hi].
 struct PagedSpan {
@@ -104,8 +102,7 @@ struct PagedOdd {
   }
 };
 
-// The kernel of many rows (paged_prefill.hip): columns of its tiles, and a launch of `tiles` of them a kv-head.
-int paged_block_cols(int head_dim);
-int paged_block(const PagedAttn& a, const ti_paged_cache* c, long tiles, hipStream_t s);
+// The kernel of many rows (paged_prefill.hip): a launch of `tiles` tiles a kv-head, of 32 columns for each of `waves` (4, 8) waves.
+int paged_block_run(const PagedAttn& a, const ti_paged_cache* c, int waves, long tiles, hipStream_t s);
 
 }  // namespace ti

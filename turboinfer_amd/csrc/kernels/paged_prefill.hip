@@ -22,9 +22,9 @@ __device__ __forceinline__ f32x16 pmma32(f16x8 a, f16x8 b, f32x16 c) { return __
 __device__ __forceinline__ f32x16 pmma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 constexpr int kBlockKeys = 64;
-template <int D>
+template <int D, int NW>   // NW: waves
 struct BlockForm {
-  static constexpr int NW = D == 256 ? 4 : 8, NT = 64 * NW, COLS = 32 * NW;
+  static constexpr int NT = 64 * NW, COLS = 32 * NW;
   static constexpr int CH = D / 8, NP = kBlockKeys * CH / NT, RP = NT / CH;   // 16-byte chunks a row; a thread's chunks; rows of a pass
   static constexpr int kTile = kBlockKeys * D * 2, kLds = 4 * kTile;         // bytes: K and V, two steps
 };
@@ -34,15 +34,15 @@ __device__ __forceinline__ int key_at(int r, int c) { return r * (2 * D) + ((c ^
 template <int D>
 __device__ __forceinline__ int value_at(int r, int c) { return r * (2 * D) + ((((c >> 1) ^ (D == 64 ? (r >> 1) & 3 : r & 7)) << 5) | (c & 1) << 4); }
 
-template <int D, class T, bool I8>
-__global__ __launch_bounds__(BlockForm<D>::NT, D == 256 ? 1 : 2) void paged_block_kernel(const PagedAttn a, const XcdDeal deal) {
-  typedef BlockForm<D> F;
+template <int D, int NW, class T, bool I8, bool SHAPED>   // SHAPED: scores with a cap or slopes
+__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(const PagedAttn a, const XcdDeal deal) {
+  typedef BlockForm<D, NW> F;
   typedef typename PagedMat<T, I8>::M M;
   typedef typename PagedMat<T, I8>::V8 V8;
   constexpr int NK = D / 16, NV = D / 32, ES = I8 ? 1 : 2;
   typedef std::conditional_t<I8, u32x2, u32x4> Raw;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ int odd, reach[4][F::NW];
+  __shared__ int odd, reach[4][NW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
   const XcdWork work = xcd_work(deal, a.q, a.out);
   if (work.head < 0) return;
@@ -109,11 +109,11 @@ __global__ __launch_bounds__(BlockForm<D>::NT, D == 256 ? 1 : 2) void paged_bloc
         for (int e = 0; e < 8; ++e) qf[k][e] = (M)(__builtin_bit_cast(float, (uint32_t)(raw[k][e] ^ flip) << 16) * up);
     }
   }
-  const float slope = a.slopes && live ? a.slopes[head] * kPagedLog2e : 0.0f;
-  __syncthreads();
+  const float slope = SHAPED && a.slopes && live ? a.slopes[head] * kPagedLog2e : 0.0f;
+  lds_sync();
   int wg_lo = INT32_MAX, wg_hi = -1, wg_lo_all = 0, wg_hi_all = INT32_MAX;
 #pragma unroll
-  for (int w = 0; w < F::NW; ++w) {
+  for (int w = 0; w < NW; ++w) {
     wg_lo = min(wg_lo, reach[0][w]);
     wg_hi = max(wg_hi, reach[1][w]);
     wg_lo_all = max(wg_lo_all, reach[2][w]);
@@ -150,6 +150,8 @@ __global__ __launch_bounds__(BlockForm<D>::NT, D == 256 ? 1 : 2) void paged_bloc
       }
     }
   };
+  // when a step's successor goes to LDS: behind its keys' products, or (long softmaxes, which it would stand in front of) at its end
+  constexpr bool late = D == 256 || SHAPED;
   Raw rk[F::NP], rv[F::NP];
   const int t_row = threadIdx.x / F::CH, t_ch = threadIdx.x % F::CH;
   auto load = [&](int step) {   // this thread's chunks of a step's keys and values
@@ -229,8 +231,10 @@ __global__ __launch_bounds__(BlockForm<D>::NT, D == 256 ? 1 : 2) void paged_bloc
 #pragma unroll
         for (int t = 0; t < 2; ++t) sc[t] = pmma32(__builtin_bit_cast(V8, *(const u32x4*)(st + key_at<D>(32 * t + c, 2 * k + h))), qf[k], sc[t]);
     }
-    store(step + 1);
-    load(step + 2);
+    if (!late || !act) {
+      store(step + 1);
+      load(step + 2);
+    }
     if (!act) continue;
     int ids[4];
     float fk[4], vl[4], vi[4];
@@ -261,17 +265,17 @@ __global__ __launch_bounds__(BlockForm<D>::NT, D == 256 ? 1 : 2) void paged_bloc
         }
       }
     }
-    // exponents of 2: mul[block] s + add[block], or s itself where a cap or a slope makes them
+    // exponents of 2: mul[block] s + add[block]
     float mul[4], add[4], mx = -INFINITY;
-    if (a.cap != 0.0f || a.slopes) {
-      if (a.cap != 0.0f) {
+    if (SHAPED && a.cap != 0.0f) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[t][i] = paged_capped(sc[t][i], fk[2 * t + (i >> 3)], a.cap);
+        for (int i = 0; i < 16; ++i) sc[t][i] = paged_capped(sc[t][i], fk[2 * t + (i >> 3)]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) fk[t] = 1.0f;
-      }
+      for (int t = 0; t < 4; ++t) fk[t] = a.cap;
+    }
+    if (SHAPED && a.slopes) {
       const float base = slope * (float)(key0 + 4 * h - p);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -353,6 +357,10 @@ __global__ __launch_bounds__(BlockForm<D>::NT, D == 256 ? 1 : 2) void paged_bloc
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int v = 0; v < NV; ++v) o[v] = pmma32(__builtin_bit_cast(V8, frag(u, v)), pf[u >> 1][u & 1], o[v]);
+    if (late) {
+      store(step + 1);
+      load(step + 2);
+    }
   }
   if constexpr (!I8) {
     lds_sync();
@@ -399,27 +407,34 @@ __global__ __launch_bounds__(BlockForm<D>::NT, D == 256 ? 1 : 2) void paged_bloc
     }
 }
 
-int paged_block_cols(int head_dim) { return head_dim == 256 ? BlockForm<256>::COLS : BlockForm<128>::COLS; }
-
-template <int D, class T>
-static int launch(const PagedAttn& a, long tiles, bool i8, hipStream_t s) {
-  auto* fn = i8 ? paged_block_kernel<D, T, true> : paged_block_kernel<D, T, false>;
+template <int D, int NW, class T>
+static int launch_waves(const PagedAttn& a, long tiles, bool i8, hipStream_t s) {
+  const bool shaped = a.cap != 0.0f || a.slopes;
+  auto* fn = i8 ? shaped ? paged_block_kernel<D, NW, T, true, true> : paged_block_kernel<D, NW, T, true, false>
+                : shaped ? paged_block_kernel<D, NW, T, false, true> : paged_block_kernel<D, NW, T, false, false>;
   // (more than 64 KiB of LDS: said once per device)
-  static std::atomic<uint64_t> said[2];
+  static std::atomic<uint64_t> said[4];
+  const int which = 2 * i8 + shaped;
   int dev = 0;
   TI_HIP_CHECK(hipGetDevice(&dev), "hipGetDevice");
-  if (!(said[i8].load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
-    TI_HIP_CHECK(hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, BlockForm<D>::kLds), "hipFuncSetAttribute");
-    said[i8].fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+  if (!(said[which].load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+    TI_HIP_CHECK(hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, BlockForm<D, NW>::kLds), "hipFuncSetAttribute");
+    said[which].fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
   }
   const XcdDeal deal = xcd_deal(a.c.s.kv_heads, (int)(tiles * a.splits));
-  hipLaunchKernelGGL(fn, xcd_grid(deal), dim3(BlockForm<D>::NT), BlockForm<D>::kLds, s, a, deal);
+  hipLaunchKernelGGL(fn, xcd_grid(deal), dim3(64 * NW), (BlockForm<D, NW>::kLds), s, a, deal);
   TI_LAUNCH_CHECK("paged_block_kernel");
   return TI_OK;
 }
+template <int D, class T>
+static int launch(const PagedAttn& a, int waves, long tiles, bool i8, hipStream_t s) {
+  if constexpr (D < 256)
+    if (waves == 8) return launch_waves<D, 8, T>(a, tiles, i8, s);
+  return launch_waves<D, 4, T>(a, tiles, i8, s);
+}
 
-int paged_block(const PagedAttn& a, const ti_paged_cache* c, long tiles, hipStream_t s) {
-  return TI_PAGED_FORM(c, launch, a, tiles, c->kv_type == TI_KV_I8, s);
+int paged_block_run(const PagedAttn& a, const ti_paged_cache* c, int waves, long tiles, hipStream_t s) {
+  return TI_PAGED_FORM(c, launch, a, waves, tiles, c->kv_type == TI_KV_I8, s);
 }
 
 }  // namespace ti

@@ -58,7 +58,7 @@ struct StreamLds {
 
 // One tile of a sequence over some of its keys: steps u0 .. u1 - 1 of 32, counted from the tile's first (u1 < 0: split u0's part of all).
 // Sums go to part `at` of a row's head, or (a.splits 1) the result to `out`.
-template <int D, class T, bool I8>
+template <int D, class T, bool I8, bool AHEAD>   // AHEAD: the next step's loads stand in front of a step's products
 __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_lds, const PagedSeq& s, long tile, int kvh, int u0, int u1, long slot) {
   typedef typename PagedMat<T, I8>::M M;
   typedef typename PagedMat<T, I8>::V8 V8;
@@ -287,13 +287,21 @@ __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_
 #pragma unroll
         for (int t = 0; t < DV; ++t) o[t] = pmma(__builtin_bit_cast(V8, frag(t)), pf, o[t]);
       };
-      Raw x0, x1;
-      load(0, x0);
-      for (int i = 0; i < n; i += 2) {
-        load(i + 1, x1);
-        compute(i, x0);
-        load(i + 2, x0);
-        if (i + 1 < n) compute(i + 1, x1);
+      if constexpr (AHEAD) {
+        Raw x0, x1;
+        load(0, x0);
+        for (int i = 0; i < n; i += 2) {
+          load(i + 1, x1);
+          compute(i, x0);
+          load(i + 2, x0);
+          if (i + 1 < n) compute(i + 1, x1);
+        }
+      } else {
+        Raw x0;
+        for (int i = 0; i < n; ++i) {
+          load(i, x0);
+          compute(i, x0);
+        }
       }
     }
   }
@@ -349,9 +357,10 @@ __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_
   }
 }
 
-// Grid (tiles, kv-heads, splits).
+// Grid (tiles, kv-heads, splits).  Steps are few: more waves a CU instead of the next step's loads in flight (us, 46 x 30 - 84 keys, 32 heads on 32: dims of
+// 128 18.6 -> 13.8, 256 52.6 -> 34.0, in int8 45.8 -> 25.0; 64 x 145 - 200 of 128 dims 42.6 -> 38.1).
 template <int D, class T, bool I8>
-__global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_stream_kernel(const PagedAttn a) {
+__global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 2 : 3) void paged_stream_kernel(const PagedAttn a) {
   __shared__ StreamLds<D> lds;
   const int per_seq = (a.G + 15) >> 4;
   const int b = a.r.start ? paged_find(a.c.seqs, blockIdx.x, [&](int j) { return paged_tile0((long)a.r.start[j] * a.G, j, 16); })
@@ -359,7 +368,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_str
   const PagedSeq s = paged_seq(a.c, a.r, b);
   const long tile = a.r.start ? blockIdx.x - paged_tile0((long)s.row0 * a.G, b, 16) : (int)blockIdx.x - b * per_seq;
   if (tile < 0 || tile * 16 >= (long)s.n * a.G) return;
-  stream_tile<D, T, I8>(a, lds, s, tile, blockIdx.y, blockIdx.z, -1, blockIdx.z);
+  stream_tile<D, T, I8, false>(a, lds, s, tile, blockIdx.y, blockIdx.z, -1, blockIdx.z);
 }
 
 // Single tokens: steps of 32 keys that sequence b's row sees.
@@ -390,7 +399,7 @@ __device__ __forceinline__ long deal_run(const PagedAttn& a, long all) { return 
 // query heads).  Part w + b of a head is workgroup w's of sequence b: each differs from the one in front by 1 in
 // w or more in b.
 template <int D, class T, bool I8>
-__global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_deal_kernel(const PagedAttn a) {
+__global__ __launch_bounds__(64 * kStreamWaves, D == 256 && !I8 ? 1 : 2) void paged_deal_kernel(const PagedAttn a) {
   __shared__ StreamLds<D> lds;
   const int lane = threadIdx.x & 63, w = blockIdx.x, per_seq = (a.G + 15) >> 4, kvh = blockIdx.y / per_seq, tile = blockIdx.y - kvh * per_seq;
   int mine = lane < a.c.seqs ? decode_steps(a, lane) : 0;
@@ -420,7 +429,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 1 : 2) void paged_dea
   }
   base = uniform(base);
   for (; n > 0; n = b < a.c.seqs ? __builtin_amdgcn_readfirstlane(decode_steps(a, b)) : 0) {
-    stream_tile<D, T, I8>(a, lds, paged_seq(a.c, a.r, b), tile, kvh, (int)(max(from, base) - base), (int)min((long)n, to - base), (long)w + b);
+    stream_tile<D, T, I8, !(D == 256 && I8)>(a, lds, paged_seq(a.c, a.r, b), tile, kvh, (int)(max(from, base) - base), (int)min((long)n, to - base), (long)w + b);
     base += n;
     if (base >= to) break;
     do ++b;
@@ -551,13 +560,13 @@ static PagedPlan paged_plan(const ti_paged_cache* c, const ti_paged_attn_args* p
   if (p->row_start && per_seq >= 32) {
     // waves of a workgroup, workgroups that fill the CUs, least steps of a split
     auto form = [&](int waves, long want, long least) {
-      const int cols = 32 * waves;
+      const int cols = c->head_dim == 256 ? 128 : 32 * waves;
       const long full = (long)c->seqs * ((per_seq + cols - 1) / cols) * c->kv_heads;
       const long keys = p->window > 0 && !p->prefix ? std::min<long>(span, (long)p->window + cols) : span;
       const long most = std::max(1l, std::min(want / full, 64l)), splits = std::max(1l, std::min(most, (keys + 63) / 64 / least));
       return PagedPlan{waves, paged_tiles(columns, c->seqs, cols), (int)splits, (int)most, 0, full * splits};
     };
-    if (c->head_dim == 256) return form(4, 256, 4);
+    if (c->head_dim == 256) return form(8, 256, 4);
     // Eight waves read each block of keys from L2 and convert it once for twice the columns, two workgroups of four hide each other's
     // waits: eight for long keys and enough columns, four where prompts are short, CUs would idle, or (heads of 64 in 16 bits) three
     // workgroups of four fit a CU.  us, 8 / 4 waves, 32 heads on 8 of 128: 4000 rows 164 / 186, capped 205 / 242, 2 x 512 behind 7.5k in int8 194

@@ -24,9 +24,10 @@ __device__ __forceinline__ f32x16 pmma32(bf16x8 a, bf16x8 b, f32x16 c) { return 
 constexpr int kBlockKeys = 64;
 template <int D, int NW>   // NW: waves
 struct BlockForm {
-  static constexpr int NT = 64 * NW, COLS = 32 * NW;
+  static constexpr bool PAIR = D == 256;   // two waves a column: each half of a step's keys, and of the dimensions
+  static constexpr int NT = 64 * NW, COLS = (PAIR ? 16 : 32) * NW;
   static constexpr int CH = D / 8, NP = kBlockKeys * CH / NT, RP = NT / CH;   // 16-byte chunks a row; a thread's chunks; rows of a pass
-  static constexpr int kTile = kBlockKeys * D * 2, kLds = 4 * kTile;         // bytes: K and V, two steps
+  static constexpr int kTile = kBlockKeys * D * 2, kLds = 4 * kTile + (PAIR ? NW * 2048 : 0);   // bytes: K and V, two steps; weights
 };
 // Chunk c of LDS row r.
 template <int D>
@@ -35,15 +36,18 @@ template <int D>
 __device__ __forceinline__ int value_at(int r, int c) { return r * (2 * D) + ((((c >> 1) ^ (D == 64 ? (r >> 1) & 3 : r & 7)) << 5) | (c & 1) << 4); }
 
 template <int D, int NW, class T, bool I8, bool SHAPED>   // SHAPED: scores with a cap or slopes
-__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(const PagedAttn a, const XcdDeal deal) {
+__global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_kernel(const PagedAttn a, const XcdDeal deal) {
   typedef BlockForm<D, NW> F;
   typedef typename PagedMat<T, I8>::M M;
   typedef typename PagedMat<T, I8>::V8 V8;
-  constexpr int NK = D / 16, NV = D / 32, ES = I8 ? 1 : 2;
+  constexpr bool PAIR = F::PAIR;
+  constexpr int NK = D / 16, NV = D / (PAIR ? 64 : 32), KT = PAIR ? 1 : 2, ES = I8 ? 1 : 2;   // this wave's: tiles of dimensions, of keys
   typedef std::conditional_t<I8, u32x2, u32x4> Raw;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ int odd, reach[4][NW];
+  __shared__ float pair[2][PAIR ? 2 : 1][PAIR ? NW / 2 : 1][32];   // references, denominators of the halves
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
+  const int half = PAIR ? wave / (NW / 2) : 0, group = PAIR ? wave % (NW / 2) : wave;
   const XcdWork work = xcd_work(deal, a.q, a.out);
   if (work.head < 0) return;
   const int kvh = work.head, split = work.j % a.splits;
@@ -52,7 +56,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(
   const PagedSeq s = paged_seq(a.c, a.r, b);
   const long tile = at_tile - paged_tile0((long)s.row0 * a.G, b, F::COLS);
   if (tile < 0 || tile * F::COLS >= (long)s.n * a.G) return;
-  const int ci = (int)tile * F::COLS + wave * 32 + c, row = ci / a.G, head = kvh * a.G + (ci - row * a.G), m = s.row0 + row, p = s.pos0 + row;
+  const int ci = (int)tile * F::COLS + group * 32 + c, row = ci / a.G, head = kvh * a.G + (ci - row * a.G), m = s.row0 + row, p = s.pos0 + row;
   const bool live = row < s.n && p >= 0 && p < a.c.s.blocks * kPagedBlock;
   PagedSpan span = {1, 0};
   if (live) span = paged_span(a, s, m, p);
@@ -220,28 +224,32 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(
     const int key0 = step * kBlockKeys;
     const bool act = key0 <= hi_any && key0 + kBlockKeys - 1 >= lo_any;
     const char* st = lds + ((step - s0) & 1) * 2 * F::kTile;
-    f32x16 sc[2];
+    f32x16 sc[KT];
     if (act) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[t][i] = 0.0f;
 #pragma unroll
       for (int k = 0; k < NK; ++k)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) sc[t] = pmma32(__builtin_bit_cast(V8, *(const u32x4*)(st + key_at<D>(32 * t + c, 2 * k + h))), qf[k], sc[t]);
+        for (int t = 0; t < KT; ++t) sc[t] = pmma32(__builtin_bit_cast(V8, *(const u32x4*)(st + key_at<D>(32 * (t + half) + c, 2 * k + h))), qf[k], sc[t]);
     }
     if (!late || !act) {
       store(step + 1);
       load(step + 2);
     }
-    if (!act) continue;
-    int ids[4];
-    float fk[4], vl[4], vi[4];
-    const int l0 = ((step - s0) & 15) * 4;
+    if (!act) {
+      if constexpr (PAIR) lds_sync();
+      continue;
+    }
+    int ids[2 * KT], no_block = 0;
+    float fk[2 * KT], vl[2 * KT], vi[2 * KT];
+    const int l0 = ((step - s0) & 15) * 4 + 2 * half, mine = key0 + 32 * half;   // this wave's first block and key
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 2 * KT; ++t) {
       ids[t] = __builtin_amdgcn_readlane(id, l0 + t);
+      no_block |= ids[t];
       fk[t] = f;
       vl[t] = 0.0f;
       vi[t] = 1.0f;
@@ -252,33 +260,35 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(
         vi[t] = __builtin_amdgcn_rcpf(sv);
       }
     }
-    const bool ragged = key0 < lo_all || key0 + kBlockKeys - 1 > hi_all || (ids[0] | ids[1] | ids[2] | ids[3]) < 0;
-    uint32_t see[2] = {0xffff, 0xffff};
+    const bool ragged = mine < lo_all || mine + 32 * KT - 1 > hi_all || no_block < 0;
+    uint32_t see[KT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) see[t] = 0xffff;
     if (ragged) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < KT; ++t) {
         see[t] = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int j = key0 + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
+          const int j = mine + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
           if (j >= span.lo && j <= span.hi && ids[2 * t + (i >> 3)] >= 0) see[t] |= 1u << i;
         }
       }
     }
     // exponents of 2: mul[block] s + add[block]
-    float mul[4], add[4], mx = -INFINITY;
+    float mul[2 * KT], add[2 * KT], mx = -INFINITY;
     if (SHAPED && a.cap != 0.0f) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[t][i] = paged_capped(sc[t][i], fk[2 * t + (i >> 3)]);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) fk[t] = a.cap;
+      for (int t = 0; t < 2 * KT; ++t) fk[t] = a.cap;
     }
     if (SHAPED && a.slopes) {
-      const float base = slope * (float)(key0 + 4 * h - p);
+      const float base = slope * (float)(mine + 4 * h - p);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float more = fmaf(slope, (float)(32 * t + 8 * (i >> 2) + (i & 3)), base);
@@ -286,13 +296,13 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(
           sc[t][i] = fmaf(sc[t][i], fk[2 * t + (i >> 3)], more);
         }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int t = 0; t < 2 * KT; ++t) {
         mul[t] = 1.0f;
         add[t] = 0.0f;
       }
     } else {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {   // (what is masked stays -inf: a factor > 0, and none of a block that is not seen)
+      for (int t = 0; t < 2 * KT; ++t) {   // (what is masked stays -inf: a factor > 0, and none of a block that is not seen)
         const bool none = I8 && ragged && !(see[t >> 1] >> 8 * (t & 1) & 255);
         mul[t] = none ? 1.0f : fk[t] < 0x1p-120f ? 0x1p-120f : fk[t];
         add[t] = none ? 0.0f : vl[t];
@@ -300,13 +310,13 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(
     }
     if (ragged) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (!(see[t] >> i & 1)) sc[t][i] = -INFINITY;
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 2 * KT; ++t) {
       float x = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 8; ++e) x = fmaxf(x, sc[t >> 1][8 * (t & 1) + e]);
@@ -314,17 +324,25 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(
     }
     mx = xor32_max(mx);
     if constexpr (!I8) mx *= mul[0];
-    if (__builtin_amdgcn_ballot_w64(mx > mr + 15.0f) != 0) {
-      const float mn = mx > mr + 15.0f ? mx - 7.0f : mr, alpha = mn == mr ? 1.0f : __builtin_amdgcn_exp2f(mr - mn);
+    auto rescale = [&](float mn) {
+      const float alpha = mn == mr ? 1.0f : __builtin_amdgcn_exp2f(mr - mn);
       mr = mn;
       lr *= alpha;
 #pragma unroll
       for (int v = 0; v < NV; ++v) o[v] *= alpha;
+    };
+    // what this step's weights are relative to (PAIR: whole, the halves' weights move to a common one exactly)
+    float ref = mr, l_step = 0.0f;
+    if constexpr (PAIR) {
+      if (mx > mr + 15.0f) ref = floorf(mx) - 7.0f;
+    } else {
+      if (__builtin_amdgcn_ballot_w64(mx > mr + 15.0f) != 0) rescale(mx > mr + 15.0f ? mx - 7.0f : mr);
+      ref = mr;
     }
-    const float off = mr == -INFINITY ? 0.0f : mr;
-    V8 pf[2][2];   // weights of 16 keys each
+    const float off = ref == -INFINITY ? 0.0f : ref;
+    V8 pf[KT][2];   // weights of 16 keys each
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float l = 0.0f;
@@ -339,7 +357,8 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(
           pf[t][u][e + 1] = w[1];
         }
         const bool none = ragged && !(see[t] >> 8 * u & 255);   // (nothing of a block, whose scale may be NaN)
-        lr = I8 ? fmaf(l, none ? 0.0f : vi[2 * t + u], lr) : lr + l;
+        float& sum = PAIR ? l_step : lr;
+        sum = I8 ? fmaf(l, none ? 0.0f : vi[2 * t + u], sum) : sum + l;
       }
     // 8 keys of dims 32 v + c: keys 4 h .. and 8 + 4 h .. of the 16 that u says
     const int tr = ((lane & 15) >> 2) + 4 * h, tc = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
@@ -347,16 +366,49 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(
       u32x2 x[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int r = 16 * u + 8 * i + tr, byte = 64 * v + tc;
+        const int r = 16 * u + 8 * i + tr, byte = 64 * (v + half * NV) + tc;
         const char* src = st + F::kTile + value_at<D>(r, byte >> 4) + (byte & 15);
         x[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)src));
       }
       return (u32x4){x[0][0], x[0][1], x[1][0], x[1][1]};
     };
+    if constexpr (PAIR) {
+      // each half's weights and reference to the other
+      u32x4* const mail = (u32x4*)(lds + 4 * F::kTile) + group * 4 * 64 + lane;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 2; ++u) mail[(2 * half + u) * 64] = __builtin_bit_cast(u32x4, pf[0][u]);
+      pair[0][half][group][c] = ref;
+      lds_sync();
+      V8 other[2];
 #pragma unroll
-      for (int v = 0; v < NV; ++v) o[v] = pmma32(__builtin_bit_cast(V8, frag(u, v)), pf[u >> 1][u & 1], o[v]);
+      for (int u = 0; u < 2; ++u) other[u] = __builtin_bit_cast(V8, mail[(2 - 2 * half + u) * 64]);
+      const float ref_o = pair[0][1 - half][group][c], both = fmaxf(ref, ref_o);
+      if (__builtin_amdgcn_ballot_w64(both != mr || ref != ref_o) != 0) {
+        const float f0 = ref == both ? 1.0f : __builtin_amdgcn_exp2f(ref - both), f1 = ref_o == both ? 1.0f : __builtin_amdgcn_exp2f(ref_o - both);
+        rescale(both);
+        l_step *= f0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            pf[0][u][e] = (M)((float)pf[0][u][e] * f0);
+            other[u][e] = (M)((float)other[u][e] * f1);
+          }
+      }
+      lr += l_step;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          o[v] = pmma32(__builtin_bit_cast(V8, frag(2 * half + u, v)), pf[0][u], o[v]);
+          o[v] = pmma32(__builtin_bit_cast(V8, frag(2 - 2 * half + u, v)), other[u], o[v]);
+        }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int v = 0; v < NV; ++v) o[v] = pmma32(__builtin_bit_cast(V8, frag(u, v)), pf[(u >> 1) % KT][u & 1], o[v]);
+    }
     if (late) {
       store(step + 1);
       load(step + 2);
@@ -369,7 +421,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(
         if (!part_seen(key / kBlockKeys)) continue;
         const int blk = key / kPagedBlock, at = paged_block(a.c.s, a.c.table[(size_t)b * a.c.table_ld + paged_column(a.c.s, blk)], kvh, blk);
         if (at < 0 || key < span.lo || key > span.hi) continue;
-        const M* x = (const M*)a.c.v + ((size_t)at * kPagedBlock + key % kPagedBlock) * D + 4 * h;
+        const M* x = (const M*)a.c.v + ((size_t)at * kPagedBlock + key % kPagedBlock) * D + 32 * NV * half + 4 * h;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -381,12 +433,17 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(
     }
   }
   lr += lane_xor<32>(lr);
+  if constexpr (PAIR) {
+    pair[1][half][group][c] = lr;
+    lds_sync();
+    lr += pair[1][1 - half][group][c];
+  }
   if (!live) return;
   const size_t rh = (size_t)m * a.heads + head;
   if (a.splits > 1) {
     const size_t at = rh * a.splits + split;
-    if (h == 0) *(float2*)(a.part_ml + 2 * at) = make_float2(mr, lr);
-    float* po = a.part_o + at * D + 4 * h;
+    if (h == 0 && half == 0) *(float2*)(a.part_ml + 2 * at) = make_float2(mr, lr);
+    float* po = a.part_o + at * D + 32 * NV * half + 4 * h;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -394,7 +451,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_block_kernel(
     return;
   }
   const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
-  T* out = (T*)a.out + (size_t)m * a.ldo + (size_t)head * D + 4 * h;
+  T* out = (T*)a.out + (size_t)m * a.ldo + (size_t)head * D + 32 * NV * half + 4 * h;
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -429,8 +486,8 @@ static int launch_waves(const PagedAttn& a, long tiles, bool i8, hipStream_t s) 
 template <int D, class T>
 static int launch(const PagedAttn& a, int waves, long tiles, bool i8, hipStream_t s) {
   if constexpr (D < 256)
-    if (waves == 8) return launch_waves<D, 8, T>(a, tiles, i8, s);
-  return launch_waves<D, 4, T>(a, tiles, i8, s);
+    if (waves == 4) return launch_waves<D, 4, T>(a, tiles, i8, s);
+  return launch_waves<D, 8, T>(a, tiles, i8, s);
 }
 
 int paged_block_run(const PagedAttn& a, const ti_paged_cache* c, int waves, long tiles, hipStream_t s) {

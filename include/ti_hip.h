@@ -410,13 +410,14 @@ int ti_attn_prefill_set_kernel(int mode);
  * place j % page of page table[b * table_ld + j / page]; entries outside [0, pages) are holes: nothing is written there, and no
  * row sees their tokens.  A page belongs to one sequence while it is written.
  *   kv_type TI_KV_SAME: elements of `dtype`;
- *   TI_KV_I8: int8 q, value = q * scale of the token's block of 16 and head, k_scale / v_scale [pages][kv_heads][page / 16].
+ *   TI_KV_I8: int8 q, value = q * scale of the token's block of 16 and head, k_scale / v_scale [pages][kv_heads][page / 16], > 0
+ *   (NaN: the block's values are none).
  * Rows of a batch are ragged: row i of sequence b (row row_start[b] + i of the call) is its token len[b] - n_b + i, n_b =
  * row_start[b + 1] - row_start[b]; len counts the call's own rows.  row_start (device, [seqs + 1], from 0, not falling) NULL: one
  * row a sequence.  Rows behind the last sequence, and rows whose token lies outside the table (or, rotated, outside the rotation
  * table), are left as they are; keys past the table are not there.
  * head_dim 64, 128 or 256; page 16, 32, 64, 128 or 256; heads a multiple of kv_heads; pages * kv_heads * page / 16 and table_ld *
- * page below 2^31; k, v and every row 16-byte aligned.  No call reads or writes memory outside the pages of its table, copies to
+ * page below 2^31; at most 2^23 rows; k, v and every row 16-byte aligned; all memory on the current device.  No call reads or writes memory outside the pages of its table, copies to
  * the host or keeps anything for the next; all can be captured into graphs. */
 enum ti_paged_dtype { TI_PAGED_F16 = 0, TI_PAGED_BF16 = 1 };
 enum ti_kv_type { TI_KV_SAME = 0, TI_KV_I8 = 1 };
@@ -455,7 +456,7 @@ int ti_paged_read(const ti_paged_cache* c, const int32_t* row_start, int rows, v
  * kv_heads).  Row at token p scores key j
  *   s = scale * (q . k_j);  softcap > 0: s = softcap * tanh(s / softcap);  slopes: s += slopes[h] * (j - p)
  * and sees it where first[row] <= j < len, j <= p or j < prefix[sequence], and window = 0 or j > p - window.  out = sum of softmax(s)
- * v; a row that sees no key: 0.  What a row does not see does not reach it, infinities and NaN among it.  fp32 scores, sums and
+ * v; a row that sees no key: 0.  |scale| <= 1e30, softcap 0 or 1e-20 .. 1e30.  What a row does not see does not reach it, infinities and NaN among it.  fp32 scores, sums and
  * weights; weights are rounded to 16 bits (TI_KV_I8: fp16) for their products with the values.
  * ti_paged_decode: one row a sequence (rows = seqs, row_start NULL).  ti_paged_prefill: any rows.
  * max_len: about the longest sequence (0: the table's size); it shapes the work only, as ti_attn_decode's splits do.

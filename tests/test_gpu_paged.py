@@ -607,3 +607,176 @@ def test_offsets_past_32_bits(ti):
         ti.sync()
     assert all(np.array_equal(a, b) for a, b in zip(*outs))
     assert (k[pages - 2, :, 299 - 256] == 1).all() and torch.isnan(k[pages - 2, :, 300 - 256:]).all()
+
+
+# ---------------------------------------------------------------- sizes of the other kernels
+def test_decode_of_many_sequences(ti, types):
+    """More than two waves of sequences, empty ones among them, keys dealt over the workgroups."""
+    rng = np.random.RandomState(40)
+    lens = [int(x) for x in rng.randint(0, 500, 150)]
+    lens[0] = lens[64] = lens[149] = 0
+    lens[100] = 1300
+    check_attention(ti, Cache(ti, rng, lens, 1, 64, 64, *types), rng, 2, [1] * 150, "decode")
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_decode_long_of_wide_groups(ti, types, dim):
+    rng = np.random.RandomState(41)
+    check_attention(ti, Cache(ti, rng, [900, 10, 300], 2, dim, 16, *types), rng, 34, [1] * 3, "decode")
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_decode_long_masks(ti, types, dim):
+    """Windows and first keys in front of which runs begin; a row that sees nothing between two that do."""
+    rng = np.random.RandomState(42)
+    lens = [1500, 700, 30, 600]
+    check_attention(ti, Cache(ti, rng, lens, 2, dim, 32, *types, holes=[(0, 40)]), rng, 4, [1] * 4, "decode", amp=2.0, window=500, first=[5, 650, 30, 0], cap=20.0,
+                    slopes=2.0 ** -rng.uniform(2, 8, 4))
+
+
+@pytest.mark.parametrize("shaped", [False, True])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prefill_of_wide_workgroups(ti, types, dim, shaped):
+    """Eight waves, keys in 32 splits of which most are empty."""
+    rng = np.random.RandomState(43)
+    cache = Cache(ti, rng, [330], 8, dim, 16, *types, room=2064)
+    more = dict(cap=6.0, slopes=2.0 ** -rng.uniform(2, 8, 8), window=150) if shaped else {}
+    check_attention(ti, cache, rng, 8, [256], amp=2.0, max_len=8192, **more)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("hint", [0, 8192])
+def test_values_that_are_no_numbers_in_shared_blocks(ti, dtype, dim, hint):
+    """An infinite and a NaN value reach the rows that see them, in their dimensions."""
+    rng = np.random.RandomState(44)
+    n = 256
+    cache = Cache(ti, rng, [n + 30], 8, dim, 32, dtype, "same", room=2080)
+    x, bits = rows16(rng, n, 8 * dim, dtype)
+    cache.upload()
+    clean = from_bits(attend(ti, cache, bits, 8, [n], max_len=hint), dtype).reshape(n, 8, dim)
+    for j, d, v in ((100, 7, np.inf), (200, dim - 3, np.nan), (220, 70, -np.inf)):
+        cache.v[cache.table[0, j // 32], 3, j % 32, d] = v
+    cache.upload()
+    got = from_bits(attend(ti, cache, bits, 8, [n], max_len=hint), dtype).reshape(n, 8, dim)
+    pos = np.arange(30, n + 30)
+    same = np.ones(got.shape, bool)
+    for j, d in ((100, 7), (200, dim - 3), (220, 70)):
+        same[pos >= j, 3, d] = False
+    assert np.array_equal(got[same], clean[same])
+    assert (got[pos >= 100, 3, 7] == np.inf).all() and np.isnan(got[pos >= 200, 3, dim - 3]).all() and (got[pos >= 220, 3, 70] == -np.inf).all()
+
+
+def test_append_and_read_of_many_rows(ti, types):
+    rng = np.random.RandomState(45)
+    new, lens = [700, 0, 433], [705, 3, 440]
+    cache = Cache(ti, rng, [l - n for l, n in zip(lens, new)], 2, 64, 128, *types, room=720)
+    cache.lens = np.asarray(lens, np.int32)
+    check_append(ti, cache, rng, new, 4, True, 64)
+
+
+def test_append_of_many_sequences(ti, types):
+    rng = np.random.RandomState(46)
+    new = [int(x) for x in rng.randint(0, 4, 150)]
+    lens = [n + int(x) for n, x in zip(new, rng.randint(0, 40, 150))]
+    cache = Cache(ti, rng, [l - n for l, n in zip(lens, new)], 1, 64, 16, *types, room=48)
+    cache.lens = np.asarray(lens, np.int32)
+    check_append(ti, cache, rng, new, 2, False, 32, True)
+
+
+def test_pages_that_sequences_share(ti, types):
+    """A common prefix in the same pages, read by three sequences."""
+    rng = np.random.RandomState(47)
+    cache = Cache(ti, rng, [400, 300, 270], 2, 64, 64, *types)
+    cache.table[1:, :4] = cache.table[0, :4]
+    check_attention(ti, cache, rng, 4, [1] * 3, "decode")
+    check_attention(ti, cache, rng, 4, [100, 20, 14])
+
+
+@pytest.mark.parametrize("fn", ["decode", "prefill"])
+def test_extreme_bounds(ti, types, fn):
+    """First keys, prefixes and windows at the ends of their type."""
+    rng = np.random.RandomState(48)
+    lo, hi = -2 ** 31, 2 ** 31 - 1
+    new = [1] * 4 if fn == "decode" else [40, 1, 30, 9]
+    cache = Cache(ti, rng, [50, 60, 30, 9], 1, 64, 16, *types)
+    rows = sum(new)
+    check_attention(ti, cache, rng, 2, new, fn, first=[(lo, hi, 0)[i % 3] for i in range(rows)], prefix=[lo, hi, 0, -1], window=hi)
+    check_attention(ti, cache, rng, 2, new, fn, prefix=[hi, lo, 1, 2])
+
+
+def test_two_streams_at_once(ti, types):
+    """Calls on two streams, each with its own workspace, as one after the other."""
+    import torch
+    rng = np.random.RandomState(49)
+    L, heads, D = ti.lib(), 8, 64
+    caches = [Cache(ti, rng, [n, 700], 2, D, 32, *types, room=1024) for n in (1000, 900)]
+    jobs = []
+    for cache in caches:
+        ref = cache.upload()
+        x, bits = rows16(rng, 62, heads * D, types[0])
+        q = upload(ti, bits)
+        start = upload(ti, starts([60, 2]))
+        for fn, rows in (("decode", 2), ("prefill", 62)):
+            out = torch.zeros(rows, heads * D, dtype=torch.int16, device="cuda")
+            a = ti.PagedAttnArgs(q=q.ptr, out=out.data_ptr(), row_start=start.ptr if fn == "prefill" else None, rows=rows, heads=heads, ldq=heads * D, ldo=heads * D, scale=D ** -0.5)
+            n = L.ti_paged_workspace_bytes(ref, C.byref(a))
+            assert n > 0
+            ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n
+            jobs.append((cache, a, out, ws, q, start, L.ti_paged_decode if fn == "decode" else L.ti_paged_prefill))
+    torch.cuda.synchronize()
+    alone = []
+    for cache, a, out, _, _, _, fn in jobs:
+        ti.check(fn(C.byref(cache.c), C.byref(a), None))
+        ti.sync()
+        alone.append(out.clone())
+        out.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for i, (cache, a, *_, fn) in enumerate(jobs):
+            ti.check(fn(C.byref(cache.c), C.byref(a), streams[i // 2].cuda_stream))
+    torch.cuda.synchronize()
+    for (_, _, out, *_), want in zip(jobs, alone):
+        assert torch.equal(out, want) and (out != 0).any()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_captured_prompts(ti, types, dim):
+    """Append and prompt attention of a chunk captured once and replayed for the chunks that follow, with eager calls between."""
+    import torch
+    rng = np.random.RandomState(50)
+    heads, kvh, B, n = 8, 2, 2, 70
+    cache = Cache(ti, rng, [0, 0], kvh, dim, 32, *types, room=512)
+    cache.upload()
+    L, w = ti.lib(), (heads + 2 * kvh) * dim
+    x = torch.zeros(B * n, w, device="cuda")
+    q, out = (torch.zeros(B * n, heads * dim, dtype=torch.int16, device="cuda") for _ in range(2))
+    lens, start = torch.tensor([n, n], dtype=torch.int32, device="cuda"), torch.tensor([0, n, 2 * n], dtype=torch.int32, device="cuda")
+    cache.c.len = lens.data_ptr()
+    a = ti.PagedAppendArgs(x=x.data_ptr(), q=q.data_ptr(), row_start=start.data_ptr(), rows=B * n, heads=heads, ldx=w, ldq=heads * dim, x_f32=1)
+    t = ti.PagedAttnArgs(q=q.data_ptr(), out=out.data_ptr(), row_start=start.data_ptr(), rows=B * n, heads=heads, ldq=heads * dim, ldo=heads * dim, scale=dim ** -0.5)
+    size = L.ti_paged_workspace_bytes(C.byref(cache.c), C.byref(t))
+    ws = torch.full((max(size, 16),), 255, dtype=torch.uint8, device="cuda")
+    t.workspace, t.workspace_bytes = ws.data_ptr(), size
+
+    def step():
+        s = torch.cuda.current_stream().cuda_stream
+        ti.check(L.ti_paged_append(C.byref(cache.c), C.byref(a), s))
+        ti.check(L.ti_paged_prefill(C.byref(cache.c), C.byref(t), s))
+
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):   # (the first call of its kind may be a captured one)
+        step()
+    for i in range(5):
+        x.copy_(torch.from_numpy(rng.standard_normal((B * n, w)).astype(np.float32)))
+        g.replay()
+        torch.cuda.synchronize()
+        replayed = out.clone()
+        out.zero_()
+        step()
+        torch.cuda.synchronize()
+        assert torch.equal(out, replayed) and (out != 0).any()
+        lens += torch.tensor([n, n - 3], dtype=torch.int32, device="cuda")

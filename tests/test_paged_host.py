@@ -118,7 +118,7 @@ def test_refused_attention(L):
     c = _cache()
     good = dict(q=4096, out=4096, rows=3, heads=4, ldq=256, ldo=256, scale=0.125)
     for bad in (dict(q=None), dict(out=None), dict(rows=4), dict(rows=-1), dict(heads=0), dict(heads=5), dict(ldq=248), dict(ldo=260), dict(q=4104), dict(out=4104),
-                dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(scale=float("nan")), dict(scale=float("inf")), dict(window=-1),
+                dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=2e30), dict(softcap=1e-30), dict(softcap=1e31), dict(rows=2 ** 23 + 1), dict(window=-1),
                 dict(max_len=-1), dict(slopes=4098), dict(first=4098), dict(prefix=4098), dict(workspace=4104)):
         for fn in (L.ti_paged_decode, L.ti_paged_prefill):
             assert fn(c, T.PagedAttnArgs(**(good | bad)), None) == 1, bad
@@ -132,3 +132,20 @@ def test_refused_attention(L):
     assert L.ti_paged_decode(c, a, None) == 1 and b"workspace" in L.ti_last_error()
     a.workspace, a.workspace_bytes = 4096, 64
     assert L.ti_paged_decode(c, a, None) == 1 and b"workspace" in L.ti_last_error()
+
+
+def test_workspace_of_any_length_serves(L):
+    """ti_paged_workspace_bytes holds for every length that a call of the same arguments names (refused for its null rows, not for its workspace)."""
+    rng = random.Random(5)
+    for i in range(3000):
+        kv_heads, G, dim = rng.choice([1, 2, 4, 8, 10, 32]), rng.choice([1, 2, 4, 5, 8, 20]), rng.choice([64, 128, 256])
+        seqs = rng.choice([1, 2, 5, 12, 50, 300])
+        c = _cache(kv_heads=kv_heads, head_dim=dim, seqs=seqs, table_ld=rng.choice([1, 16, 200, 3000]), pages=100, kv_type=rng.choice([T.KV_SAME, T.KV_I8]))
+        rows = seqs if i % 3 == 0 else rng.randrange(1, 5000)
+        a = T.PagedAttnArgs(rows=rows, heads=kv_heads * G, ldq=kv_heads * G * dim, ldo=kv_heads * G * dim, scale=1.0, row_start=None if i % 3 == 0 else 4096,
+                            prefix=rng.choice([None, 4096]), window=rng.choice([0, 100, 3000]))
+        n = L.ti_paged_workspace_bytes(c, a)
+        a.workspace, a.workspace_bytes = 4096, n
+        for max_len in (0, 1, 200, 300, 1000, 1536, 2047, 2048, 5000, 48000, 10 ** 6):
+            a.max_len = max_len
+            assert L.ti_paged_prefill(c, a, None) == 1 and b"null pointer" in L.ti_last_error(), (L.ti_last_error(), rows, seqs, kv_heads, G, dim, c.table_ld, max_len)

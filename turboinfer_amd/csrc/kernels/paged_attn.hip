@@ -572,8 +572,10 @@ static PagedPlan paged_plan(const ti_paged_cache* c, const ti_paged_attn_args* p
     // workgroups of four fit a CU.  us, 8 / 4 waves, 32 heads on 8 of 128: 4000 rows 164 / 186, capped 205 / 242, 2 x 512 behind 7.5k in int8 194
     // / 216, 128 behind 32k int8 108 / 126, 256 behind 8k 57 / 62; 1000 rows 38.6 / 37.8, 12 prompts of 40 - 640 60 / 54, 8 x 200 rows of 32 heads on
     // 32 41 / 24, 64 x 64 rows 54 / 39; 512 rows 31 / 25 (64 workgroups of eight); heads of 64, 4000 rows 111 / 103, int8 130 / 149.
-    const PagedPlan wide = form(8, 256, 4);
-    return !(c->head_dim == 64 && c->kv_type == TI_KV_SAME) && per_seq >= 192 && span >= 2048 && wide.filled >= 192 ? wide : form(4, 512, 8);
+    const PagedPlan wide = form(8, 256, 4), narrow = form(4, 512, 8);
+    PagedPlan plan = !(c->head_dim == 64 && c->kv_type == TI_KV_SAME) && per_seq >= 192 && span >= 2048 && wide.filled >= 192 ? wide : narrow;
+    plan.most = std::max(wide.most, narrow.most);
+    return plan;
   }
   if (p->window > 0 && !p->prefix) span = std::min<long>(span, (long)p->window + 16);
   const long tiles = p->row_start ? paged_tiles(columns, c->seqs, 16) : (long)c->seqs * ((G + 15) / 16);
@@ -622,18 +624,24 @@ static size_t part_bytes(const ti_paged_cache* c, size_t n) { return n * ((size_
 static int check_attn(const ti_paged_cache* c, const ti_paged_attn_args* p, const char* who) {
   if (const int rc = ti_paged_check(c, who)) return rc;
   if (!p) return ti_set_error(TI_ERR_ARG, "%s: null arguments", who);
-  if (p->rows < 0 || p->rows > (1 << 24) || p->heads < 1 || p->heads > 16384 || p->heads % c->kv_heads || p->max_len < 0 || p->window < 0)
+  if (p->rows < 0 || p->rows > kPagedRows || p->heads < 1 || p->heads > 16384 || p->heads % c->kv_heads || p->max_len < 0 || p->window < 0)
     return ti_set_error(TI_ERR_ARG, "%s: bad sizes rows=%d heads=%d kv_heads=%d max_len=%d window=%d", who, p->rows, p->heads, c->kv_heads,
                         p->max_len, p->window);
   if (!p->row_start && p->rows != c->seqs) return ti_set_error(TI_ERR_ARG, "%s: %d rows of %d sequences without row_start", who, p->rows, c->seqs);
   if ((int64_t)p->rows * p->heads > INT32_MAX) return ti_set_error(TI_ERR_ARG, "%s: %d rows of %d heads in a call", who, p->rows, p->heads);
-  if (!(p->softcap >= 0.0f) || !(p->softcap < 3e38f) || !(fabsf(p->scale) < 3e38f))
+  if (!(p->softcap == 0.0f || (p->softcap >= 1e-20f && p->softcap <= 1e30f)) || !(fabsf(p->scale) <= 1e30f))
     return ti_set_error(TI_ERR_ARG, "%s: scale %g, softcap %g", who, (double)p->scale, (double)p->softcap);
   return TI_OK;
 }
 
 static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_stream_t stream_, const char* who) {
   if (const int rc = check_attn(c, p, who)) return rc;
+  const PagedPlan plan = paged_plan(c, p);
+  if (plan.tiles > (1 << 23) || (int64_t)plan.tiles * plan.splits * c->kv_heads > INT32_MAX)
+    return ti_set_error(TI_ERR_ARG, "%s: %d rows of %d sequences and %d heads in a call", who, p->rows, c->seqs, p->heads);
+  const size_t n = parts(c, p, plan, plan.splits), need = part_bytes(c, n);
+  if (need && (!p->workspace || p->workspace_bytes < (int64_t)need))
+    return ti_set_error(TI_ERR_ARG, "%s: workspace of %ld bytes, %zu needed", who, (long)(p->workspace ? p->workspace_bytes : 0), need);
   if (!p->q || !p->out) return ti_set_error(TI_ERR_ARG, "%s: null pointer", who);
   const int64_t w = (int64_t)p->heads * c->head_dim;
   if (p->ldq < w || p->ldo < w || p->ldq % 8 || p->ldo % 8 || ((uintptr_t)p->q | (uintptr_t)p->out) % 16)
@@ -641,10 +649,6 @@ static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_strea
   if (((uintptr_t)p->row_start | (uintptr_t)p->slopes | (uintptr_t)p->first | (uintptr_t)p->prefix) % 4 || (uintptr_t)p->workspace % 16)
     return ti_set_error(TI_ERR_ARG, "%s: pointers are not aligned", who);
   if (p->rows == 0) return TI_OK;
-  const PagedPlan plan = paged_plan(c, p);
-  const size_t n = parts(c, p, plan, plan.splits), need = part_bytes(c, n);
-  if (need && (!p->workspace || p->workspace_bytes < (int64_t)need))
-    return ti_set_error(TI_ERR_ARG, "%s: workspace of %ld bytes, %zu needed", who, (long)(p->workspace ? p->workspace_bytes : 0), need);
   float* ws = (float*)p->workspace;
   const float cap = p->softcap;
   const PagedAttn a = {ti_paged_form(c), {p->row_start, p->rows}, p->q, p->out, p->slopes, p->first, p->prefix, n ? ws : nullptr,

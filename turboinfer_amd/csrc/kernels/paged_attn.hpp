@@ -55,7 +55,7 @@ struct PagedSpan {
 __device__ __forceinline__ PagedSpan paged_span(const PagedAttn& a, const PagedSeq& s, int m, int p) {
   int lo = a.window > 0 ? p - a.window + 1 : 0, hi = p;
   if (a.first) lo = max(lo, a.first[m]);
-  if (a.prefix) hi = max(hi, a.prefix[s.b] - 1);
+  if (a.prefix) hi = max(hi, max(a.prefix[s.b], 0) - 1);
   return {max(lo, 0), min(hi, s.len - 1)};
 }
 

@@ -228,7 +228,7 @@ int append(AppendArgs a, const ti_paged_cache* c, int x_f32, hipStream_t s) {
   if (a.r.rows >= 1024 && a.row_parts > 1) a.row_parts = 1;
   const long slots = !i8 ? 0 : a.r.start ? paged_touches(a.r.rows, c->seqs) : a.r.rows;
   const long grid = (long)a.r.rows * a.row_parts + slots * 2 * c->kv_heads;
-  if (grid > INT32_MAX) return ti_set_error(TI_ERR_ARG, "ti_paged_append: %d rows of %d heads in a call", a.r.rows, a.heads + 2 * c->kv_heads);
+  if (grid > UINT32_MAX / (2 * D)) return ti_set_error(TI_ERR_ARG, "ti_paged_append: %d rows of %d heads in a call", a.r.rows, a.heads + 2 * c->kv_heads);
   auto* fn = i8 ? (x_f32 ? paged_append_kernel<D, T, float, true> : paged_append_kernel<D, T, T, true>)
                 : (x_f32 ? paged_append_kernel<D, T, float, false> : paged_append_kernel<D, T, T, false>);
   hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(2 * D), 0, s, a);
@@ -278,7 +278,7 @@ ti::PagedCache ti_paged_form(const ti_paged_cache* c) {
 
 // Rows of a call: TI_OK, or the error set.
 static int check_rows(const ti_paged_cache* c, const int32_t* start, int rows, const char* who) {
-  if (rows < 0 || rows > (1 << 24)) return ti_set_error(TI_ERR_ARG, "%s: rows=%d", who, rows);
+  if (rows < 0 || rows > ti::kPagedRows) return ti_set_error(TI_ERR_ARG, "%s: rows=%d", who, rows);
   if (!start && rows != c->seqs) return ti_set_error(TI_ERR_ARG, "%s: %d rows of %d sequences without row_start", who, rows, c->seqs);
   if (!ti::aligned(start, 4)) return ti_set_error(TI_ERR_ARG, "%s: row_start is not aligned", who);
   return TI_OK;

@@ -61,13 +61,14 @@ __device__ __forceinline__ u16x8 pack8(const float* v) {
   return __builtin_bit_cast(u16x8, o);
 }
 
-}  // namespace ti
-
 // fn<D, T>(args ..) of the cache's sizes
 #define TI_PAGED_FORM(c, fn, ...)                                                                                     \
   ((c)->dtype == TI_PAGED_F16                                                                                        \
        ? (c)->head_dim == 64 ? fn<64, f16>(__VA_ARGS__) : (c)->head_dim == 128 ? fn<128, f16>(__VA_ARGS__) : fn<256, f16>(__VA_ARGS__) \
        : (c)->head_dim == 64 ? fn<64, bf16>(__VA_ARGS__) : (c)->head_dim == 128 ? fn<128, bf16>(__VA_ARGS__) : fn<256, bf16>(__VA_ARGS__))
+
+constexpr int kPagedRows = 1 << 23;   // of a call
+}  // namespace ti
 
 // Checks of a cache's description (TI_OK, or the error set), and its kernels' form.
 extern "C++" int ti_paged_check(const ti_paged_cache* c, const char* who);

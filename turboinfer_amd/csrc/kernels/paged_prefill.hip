@@ -234,6 +234,15 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
       for (int k = 0; k < NK; ++k)
 #pragma unroll
         for (int t = 0; t < KT; ++t) sc[t] = pmma32(__builtin_bit_cast(V8, *(const u32x4*)(st + key_at<D>(32 * (t + half) + c, 2 * k + h))), qf[k], sc[t]);
+      if constexpr (!PAIR) {   // four keys' fragments on their way in front of the products (one: 4000 capped rows 203 -> 197 us)
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int i = 0; i < NK * KT - 4; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
+      }
     }
     if (!late || !act) {
       store(step + 1);

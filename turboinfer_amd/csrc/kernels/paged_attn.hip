@@ -16,7 +16,11 @@
 // int8: score (q . k) ks, ks a block's; weights are taken with the values' scale, 2^(score + log2 vs - m), so that fp16 weights stay
 // near 1 whatever vs, times exact values; the denominator gets them times 1 / vs.  Queries are scaled to fp16 by a power of 2.
 //
-// A tile's keys are cut over workgroups (grid z), by absolute length, and joined by a second launch.
+// A tile's keys are cut over workgroups, and joined by a second launch (4 - 6 us with its gap): rows' in equal splits (grid z), single tokens' as runs of
+// one list of all sequences' steps, so that long sequences keep no workgroup longer than another.
+//
+// Bound: HBM.  us and TB/s: 32 streams of 4k - 8k, 32 heads on 8 of 128, int8 87 / 4.6, f16 146 / 5.5; one of 128k int8 59 / 4.6; without any arithmetic 82, 145, 57.
+// Loads of the next step stand in front of a step's products; loading keys behind theirs, values behind theirs needs no more registers, but int8 took 99.
 #include <math.h>
 
 #include "paged_attn.hpp"
@@ -392,7 +396,7 @@ __device__ __forceinline__ unsigned wave_scan(unsigned v) {
   }
   return v;
 }
-constexpr int kDealLeast = kStreamWaves;   // steps of a run: one a wave
+constexpr int kDealLeast = 2;   // steps of a run (us, 2 / 4 / 8: one stream of 2000 keys, 32 heads on 8 11.6 / 12.4 / 12.9, of 256 dims 14.6 / 16.6 / 18.1)
 __device__ __forceinline__ long deal_run(const PagedAttn& a, long all) { return max((all + a.deal - 1) / a.deal, (long)kDealLeast); }
 
 // The steps of all sequences are one list, cut into equal runs for the a.deal workgroups of a kv-head: grid (a.deal, kv-heads * tiles of 16

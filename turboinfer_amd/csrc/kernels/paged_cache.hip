@@ -7,6 +7,10 @@
 //
 // int8: one workgroup per (block of 16 tokens, kv-head, k or v) holds the whole block in registers, finds the largest new value,
 // and writes new and moved old tokens once.
+//
+// Bound: of many rows HBM (16-bit caches, 8000 rows of 32 heads on 8 of 128: 43 us, 4.7 TB/s; read back 32000 tokens 43.6 us, 4.8 TB/s: a large copy's
+// 4.9), int8 blocks by their chain of lookup, rows, maximum (55 us for the same rows, 3.3 TB/s; several heads a workgroup with the next one's rows
+// ahead: 59); of a step its launch (32 streams 3.3 us).
 #include <math.h>
 
 #include "paged_device.hpp"

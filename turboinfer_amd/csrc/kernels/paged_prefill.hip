@@ -7,6 +7,14 @@
 //   O^T += V^T P^T  32x32x16: the lane's own 8 weights (keys 4 h .., 8 + 4 h .. of 16) are its operand; values by transposed LDS reads
 // LDS rows are rotated by their number, 16 bytes at a time (keys) or 32 (values), so that neither read meets a bank twice as often as
 // it must.  Scores, reference and sums as in paged_attn.hip.
+//
+// Heads of 256 dims: two waves have the same 32 columns, each the scores of half of a step's keys and the sums of half of the dimensions, so that both fit
+// the registers of two waves a SIMD; they hand each other their weights through LDS, with a reference each (a whole number: moving to the larger is
+// exact).  4000 rows of 16 heads on 8: 308 -> 220 us against one wave with all of it, one a SIMD.
+//
+// Bound: one issue port for matrix products and vector instructions.  4000 rows of 32 heads on 8 of 128: 156 - 166 us (790 - 840 TFLOP/s; 16000 rows 980, a
+// library product 1218), matrix units busy 36 % of the cycles, vector instructions 47 %, LDS 33 %; with a cap 197 us, 28 % and 59 %; int8 175 - 186.  Two groups of
+// waves a phase apart (one multiplies, one weighs): 195 us, 274 with a cap.
 #include <math.h>
 
 #include <atomic>

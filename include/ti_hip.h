@@ -417,7 +417,7 @@ int ti_attn_prefill_set_kernel(int mode);
  * row a sequence.  Rows behind the last sequence, and rows whose token lies outside the table (or, rotated, outside the rotation
  * table), are left as they are; keys past the table are not there.
  * head_dim 64, 128 or 256; page 16, 32, 64, 128 or 256; heads a multiple of kv_heads; pages * kv_heads * page / 16 and table_ld *
- * page below 2^31; at most 2^23 rows; k, v and every row 16-byte aligned; all memory on the current device.  No call reads or writes memory outside the pages of its table, copies to
+ * page below 2^31; at most 2^23 rows; k, v and every row 16-byte aligned; all memory on the current device, outputs apart from inputs.  No call reads or writes memory outside the pages of its table, copies to
  * the host or keeps anything for the next; all can be captured into graphs. */
 enum ti_paged_dtype { TI_PAGED_F16 = 0, TI_PAGED_BF16 = 1 };
 enum ti_kv_type { TI_KV_SAME = 0, TI_KV_I8 = 1 };

@@ -215,10 +215,10 @@ def test_holes(ti, types, fn, entry):
 def test_lengths_past_the_table(ti, types):
     """Tokens past the table are not there; their rows are left."""
     rng = np.random.RandomState(15)
-    for lens, new in (([70, 64, -5], [10, 64, 3]), ([2 ** 31 - 1, 66, -2 ** 31], [3, 4, 5]), ([2, 1, 0], [5, 1, 2])):
+    for lens, new in (([70, 64, -5], [10, 64, 3]), ([2 ** 31 - 1, 66, -2 ** 31], [3, 4, 5]), ([2, 1, 0], [5, 1, 2]), ([65, 64, 0], [1, 1, 1])):
         full = Cache(ti, np.random.RandomState(16), [64, 64, 64], 1, 64, 16, *types)   # (every place holds a token)
         full.lens = np.asarray(lens, np.int32)
-        check_attention(ti, full, rng, 2, new)
+        check_attention(ti, full, rng, 2, new, "decode" if new == [1, 1, 1] else "prefill")
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
@@ -780,3 +780,43 @@ def test_captured_prompts(ti, types, dim):
         torch.cuda.synchronize()
         assert torch.equal(out, replayed) and (out != 0).any()
         lens += torch.tensor([n, n - 3], dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("kv", ["same", "i8"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("fn", ["decode", "prefill"])
+def test_values_near_the_largest(ti, kv, dim, fn):
+    """Values up to 2e38: sums of weights times them stay inside fp32 where the result does."""
+    rng = np.random.RandomState(51)
+    new = [1] if fn == "decode" else [90]
+    cache = Cache(ti, rng, [700], 1, dim, 32, "bf16", kv)
+    if kv == "same":
+        cache.v = from_bits(bits16(np.where(np.isnan(cache.v), np.nan, np.sign(cache.v) * 2e38), "bf16"), "bf16")
+    else:
+        cache.vs = np.where(np.isnan(cache.vs), np.nan, 1.5e36).astype(np.float32)
+    check_attention(ti, cache, rng, 1, new, fn, amp=0.3)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_long_runs_of_zero_values(ti, dim):
+    """int8: 20160 tokens whose values are 0 (the least scale) before some that are not, in one workgroup's sum; their scores 8 octaves above the first ones'."""
+    rng = np.random.RandomState(52)
+    n, rows = 20224, 40
+    cache = Cache(ti, rng, [n], 1, dim, 256, "f16", "i8")
+    cache.vs[:] = np.float32(TINY)
+    cache.v[:] = 0
+    cache.k[:] = 127
+    cache.ks[:] = 1.0
+    e = cache.table[0]
+    cache.k[e[0], 0, :64] = 0
+    last = (n - 64) // 256
+    cache.v[e[last], 0, (n - 64) % 256: (n - 64) % 256 + 64] = rng.randint(-127, 128, (64, dim))
+    cache.vs[e[last], 0, (n - 64) % 256 // 16: (n - 64) % 256 // 16 + 4] = 0.01
+    x = np.full((rows, dim), 1.0)
+    bits = bits16(x, "f16")
+    cache.upload()
+    scale = 7.9 * np.log(2) / (127 * dim)
+    got = from_bits(attend(ti, cache, bits, 1, [rows], scale=scale, max_len=1), "f16")
+    ref, absv, mag, seen = attention(cache, x, [rows], 1, scale)
+    assert np.abs(ref).max() > 0
+    assert (np.abs(got - ref) <= attention_tolerance(cache, ref, absv, mag, seen)).all()

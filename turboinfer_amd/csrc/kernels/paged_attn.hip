@@ -2,7 +2,7 @@
 // paged_prefill.hip).
 //
 // o = sum_j w_j v_j / sum_j w_j, w_j = 2^(score_j - m): one pass over the keys, the running reference m moved only where a weight
-// would pass 2^15 (sums follow by 2^(m - m')).
+// would pass 2^15 (bf16: 1; PagedRef), the sums following by 2^(m - m').
 //
 // 16 columns -- (row, query head) pairs that share a kv-head -- are a tile; a workgroup's four waves take the tile's keys 32 at a
 // time in turn, straight from HBM into registers:
@@ -207,7 +207,7 @@ __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_
             ft *= __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), 2 * i + t));
             const float sv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), 2 * i + t));
             vl[t] = __builtin_amdgcn_logf(sv);
-            vi[t] = ragged && !(see >> 4 * t & 15) ? 0.0f : __builtin_amdgcn_rcpf(sv);   // (0 of a block, whose scale may be NaN)
+            vi[t] = ragged && !(see >> 4 * t & 15) ? 0.0f : __builtin_amdgcn_rcpf(sv) * kPagedUnit;   // (0 of a block, whose scale may be NaN)
           }
           if (a.cap != 0.0f) {
             asm volatile("" : "+v"(ft));
@@ -236,8 +236,9 @@ __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_
           for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][e]);
         }
         mx = xor32_max(xor16_max(mx));
-        if (__builtin_amdgcn_ballot_w64(mx > mr + 15.0f) != 0) {
-          const float mn = mx > mr + 15.0f ? mx - 7.0f : mr, alpha = mn == mr ? 1.0f : __builtin_amdgcn_exp2f(mr - mn);
+        typedef PagedRef<M> Ref;
+        if (__builtin_amdgcn_ballot_w64(mx > mr + Ref::kUp) != 0) {
+          const float mn = mx > mr + Ref::kUp ? mx + Ref::kSet : mr, alpha = mn == mr ? 1.0f : __builtin_amdgcn_exp2f(mr - mn);
           mr = mn;
           lr *= alpha;
 #pragma unroll
@@ -349,7 +350,7 @@ __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_
     for (int d = 0; d < DV; d += 4) *(f32x4*)(po + d) = (f32x4){acc[d], acc[d + 1], acc[d + 2], acc[d + 3]};
     return;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = a.unit / l;
   T* out = (T*)a.out + (size_t)(s.row0 + row_c) * a.ldo + (size_t)head_c * D + part * DV;
 #pragma unroll
   for (int d = 0; d < DV; d += 4) {
@@ -499,7 +500,7 @@ __global__ __launch_bounds__(256) void deal_join_kernel(const PagedAttn a) {
   const int d = threadIdx.x;
   l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
   const float o = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
-  ((T*)a.out)[(size_t)m * a.ldo + (size_t)head * D + d] = (T)(l == 0.0f ? 0.0f : o / l);
+  ((T*)a.out)[(size_t)m * a.ldo + (size_t)head * D + d] = (T)(l == 0.0f ? 0.0f : o * (a.unit / l));
 }
 
 // The splits of rows: D / 4 threads a (row, head), 1024 / D heads a workgroup.  Grid (rows, groups of heads).
@@ -541,7 +542,7 @@ __global__ __launch_bounds__(256) void split_join_kernel(const PagedAttn a) {
   typedef T Q4 __attribute__((ext_vector_type(4)));
   Q4 y;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = (T)(l == 0.0f ? 0.0f : acc[e] / l);
+  for (int e = 0; e < 4; ++e) y[e] = (T)(l == 0.0f ? 0.0f : acc[e] * (a.unit / l));
   *(Q4*)((T*)a.out + (size_t)m * a.ldo + (size_t)head * D + d) = y;
 }
 
@@ -657,7 +658,7 @@ static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_strea
   const float cap = p->softcap;
   const PagedAttn a = {ti_paged_form(c), {p->row_start, p->rows}, p->q, p->out, p->slopes, p->first, p->prefix, n ? ws : nullptr,
                        n ? ws + n * c->head_dim : nullptr, p->heads, p->heads / c->kv_heads, p->ldq, p->ldo, p->window, plan.splits, plan.deal,
-                       cap > 0.0f ? 2.0f * p->scale * kPagedLog2e / cap : p->scale * kPagedLog2e, 2.0f * cap * kPagedLog2e};
+                       c->kv_type == TI_KV_I8 ? kPagedUnit : 1.0f, cap > 0.0f ? 2.0f * p->scale * kPagedLog2e / cap : p->scale * kPagedLog2e, 2.0f * cap * kPagedLog2e};
   return TI_PAGED_FORM(c, launch_attn, a, plan, c, (hipStream_t)stream_);
 }
 

@@ -19,10 +19,22 @@ struct PagedAttn {
   float* part_o;    // sums of parts of the keys (NULL: none), relative to 2^part_ml[..][0]: [row][head][split][D]; dealt: [head][deal + seqs][D]
   float* part_ml;   // [..][2]: reference, denominator
   int heads, G, ldq, ldo, window, splits, deal;
+  float unit;       // of the denominators: int8 kPagedUnit, else 1
   float f, cap;     // weights are 2^(f s), or with a cap 2^(cap paged_capped(s, f))
 };
 
 constexpr float kPagedLog2e = 1.44269504088896341f;
+
+// Weights are 2^(exponent - reference).  A column's reference moves (its sums with it) where an exponent passes it by kUp, to the exponent + kSet: fp16
+// weights are at most 2^15 and the largest is at least 2^7, so that only what is 2^-21 of it loses bits; bf16 weights, whose range is fp32's, are at
+// most 1, so that sums overflow only where the result does.
+template <class M>
+struct PagedRef {
+  static constexpr bool H = std::is_same_v<M, f16>;
+  static constexpr float kUp = H ? 15.0f : 0.0f, kSet = H ? -7.0f : 8.0f;
+};
+// int8: the denominators' terms (weight / vs), at most 2^115 for the least scale, are taken 2^-12 times, the result with them: 2^24 keys fit.
+constexpr float kPagedUnit = 0x1p-12f;
 
 // Matrix operands: int8 keys and values are multiplied as fp16, which holds them exactly.
 template <class T, bool I8>

@@ -274,7 +274,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
         fk[t] *= __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), l0 + t));
         const float sv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), l0 + t));
         vl[t] = __builtin_amdgcn_logf(sv);
-        vi[t] = __builtin_amdgcn_rcpf(sv);
+        vi[t] = __builtin_amdgcn_rcpf(sv) * kPagedUnit;
       }
     }
     const bool ragged = mine < lo_all || mine + 32 * KT - 1 > hi_all || no_block < 0;
@@ -349,11 +349,12 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
       for (int v = 0; v < NV; ++v) o[v] *= alpha;
     };
     // what this step's weights are relative to (PAIR: whole, the halves' weights move to a common one exactly)
+    typedef PagedRef<M> Ref;
     float ref = mr, l_step = 0.0f;
     if constexpr (PAIR) {
-      if (mx > mr + 15.0f) ref = floorf(mx) - 7.0f;
+      if (mx > mr + Ref::kUp) ref = floorf(mx) + Ref::kSet;
     } else {
-      if (__builtin_amdgcn_ballot_w64(mx > mr + 15.0f) != 0) rescale(mx > mr + 15.0f ? mx - 7.0f : mr);
+      if (__builtin_amdgcn_ballot_w64(mx > mr + Ref::kUp) != 0) rescale(mx > mr + Ref::kUp ? mx + Ref::kSet : mr);
       ref = mr;
     }
     const float off = ref == -INFINITY ? 0.0f : ref;
@@ -467,7 +468,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
       for (int i = 0; i < 16; i += 4) *(f32x4*)(po + 32 * v + 2 * i) = (f32x4){o[v][i], o[v][i + 1], o[v][i + 2], o[v][i + 3]};
     return;
   }
-  const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+  const float inv = a.unit / lr;
   T* out = (T*)a.out + (size_t)m * a.ldo + (size_t)head * D + 32 * NV * half + 4 * h;
 #pragma unroll
   for (int v = 0; v < NV; ++v)

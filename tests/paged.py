@@ -27,6 +27,8 @@ class Cache:
     """lens: tokens of every sequence; room: tokens that its table has places for.  Places that hold no token are `garbage`
     (16-bit: NaN; int8: any values under NaN scales).  holes: {(sequence, table column)}."""
 
+    wide = 0   # tokens that tables have columns for: those behind the sequence's own name no page
+
     def __init__(self, ti, rng, lens, kv_heads, dim, page, dtype="f16", kv="same", room=None, holes=(), spare=2, amp=1.0, bad_entry=-1):
         self.ti, self.dtype, self.kv, self.page, self.kvh, self.dim = ti, dtype, kv, page, kv_heads, dim
         self.lens = np.asarray(lens, np.int32)
@@ -70,11 +72,13 @@ class Cache:
         T = self.ti
         dev = T.DeviceBuffer.from_array
         raw = (lambda x: bits16(x, self.dtype)) if self.kv == "same" else (lambda x: x.astype(np.int8))
-        self.buf = {"k": dev(raw(self.k)), "v": dev(raw(self.v)), "table": dev(self.table), "len": dev(self.lens)}
+        more = max(0, -(-self.wide // self.page) - self.table.shape[1])
+        table = np.ascontiguousarray(np.pad(self.table, ((0, 0), (0, more)), constant_values=-1))
+        self.buf = {"k": dev(raw(self.k)), "v": dev(raw(self.v)), "table": dev(table), "len": dev(self.lens)}
         if self.kv == "i8":
             self.buf |= {"ks": dev(self.ks), "vs": dev(self.vs)}
         p = lambda n: self.buf[n].ptr if n in self.buf else None  # noqa: E731
-        self.c = T.PagedCache(k=p("k"), v=p("v"), k_scale=p("ks"), v_scale=p("vs"), table=p("table"), len=p("len"), table_ld=self.table.shape[1],
+        self.c = T.PagedCache(k=p("k"), v=p("v"), k_scale=p("ks"), v_scale=p("vs"), table=p("table"), len=p("len"), table_ld=table.shape[1],
                               pages=self.pages, page=self.page, kv_heads=self.kvh, head_dim=self.dim, seqs=len(self.lens),
                               dtype=T.PAGED_F16 if self.dtype == "f16" else T.PAGED_BF16, kv_type=T.KV_SAME if self.kv == "same" else T.KV_I8)
         return C.byref(self.c)

@@ -1,0 +1,42 @@
+"""The paged cache's attention by tables that have room for much longer sequences: kernels and splits are chosen by the room, so that
+short sequences meet the ways of long ones too -- single tokens' keys dealt over the workgroups, rows' keys shared and in many splits."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from paged import Cache
+from test_gpu_paged import (check_attention, test_decode, test_decode_long, test_decode_long_masks, test_decode_long_of_wide_groups,  # noqa: F401
+                            test_decode_of_many_sequences, test_decode_queries_of_any_size, test_decode_scores_and_masks, test_decode_sharp_and_flat_rows,
+                            test_extreme_bounds, test_holes, test_int8_blocks_that_are_no_numbers, test_long_runs_of_zero_values, test_pages_that_sequences_share,
+                            test_prefill, test_prefill_behind_a_long_cache, test_prefill_groups, test_prefill_many_rows, test_prefill_scores_and_masks,
+                            test_prompts_then_steps, test_captured_prompts, test_captured_steps, test_two_streams_at_once, test_values_near_the_largest,
+                            test_values_of_many_sizes, test_values_that_are_no_numbers_in_shared_blocks, test_what_a_row_does_not_see_does_not_reach_it, types)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def wide_tables(monkeypatch):
+    monkeypatch.setattr(Cache, "wide", 70000)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_dealt_windows(ti, types, dim):
+    """Windows and first keys in front of which runs begin; a row that sees nothing between two that do."""
+    rng = np.random.RandomState(60)
+    lens = [7400, 30, 6600, 900]
+    check_attention(ti, Cache(ti, rng, lens, 1, dim, 64, *types, holes=[(0, 40)]), rng, 3, [1] * 4, "decode", amp=2.0, window=6300, first=[2000, 30, 0, 850], cap=20.0,
+                    slopes=2.0 ** -rng.uniform(8, 12, 3))
+
+
+@pytest.mark.parametrize("shaped", [False, True])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_shared_keys_in_one_split(ti, types, dim, shaped, monkeypatch):
+    """Many prompts of few rows, one workgroup a tile."""
+    monkeypatch.setattr(Cache, "wide", 0)
+    rng = np.random.RandomState(61)
+    new = [7 * i % 38 for i in range(32)]   # (18 a sequence)
+    lens = [n + int(x) for n, x in zip(new, rng.randint(0, 30, 32))]
+    more = dict(cap=6.0, slopes=2.0 ** -rng.uniform(2, 8, 16), window=20) if shaped else {}
+    check_attention(ti, Cache(ti, rng, lens, 8, dim, 16, *types), rng, 16, new, amp=2.0, **more)

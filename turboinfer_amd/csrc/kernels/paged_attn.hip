@@ -16,8 +16,8 @@
 // int8: score (q . k) ks, ks a block's; weights are taken with the values' scale, 2^(score + log2 vs - m), so that fp16 weights stay
 // near 1 whatever vs, times exact values; the denominator gets them times 1 / vs.  Queries are scaled to fp16 by a power of 2.
 //
-// A tile's keys are cut over workgroups, and joined by a second launch (4 - 6 us with its gap): rows' in equal splits (grid z), single tokens' as runs of
-// one list of all sequences' steps, so that long sequences keep no workgroup longer than another.
+// A tile's keys are cut over workgroups, and joined by a second launch (4 - 6 us with its gap): in equal splits (grid z), or, long keys of single tokens,
+// as runs of one list of all sequences' steps, so that long sequences keep no workgroup longer than another.
 //
 // Bound: HBM.  us and TB/s: 32 streams of 4k - 8k, 32 heads on 8 of 128, int8 87 / 4.6, f16 146 / 5.5; one of 128k int8 59 / 4.6; without any arithmetic 82, 145, 57.
 // Loads of the next step stand in front of a step's products; loading keys behind theirs, values behind theirs needs no more registers, but int8 took 99.
@@ -556,43 +556,54 @@ struct PagedPlan {
 };
 static PagedPlan paged_plan(const ti_paged_cache* c, const ti_paged_attn_args* p) {
   const int G = p->heads / c->kv_heads;
-  const long columns = (long)p->rows * G;
+  const long columns = (long)p->rows * G, per_seq = columns / c->seqs;
+  const bool i8 = c->kv_type == TI_KV_I8;
   long span = (long)c->table_ld * c->page;
   if (p->max_len > 0) span = std::min<long>(span, p->max_len);
-  const long per_seq = columns / c->seqs;
-  // From 32 columns a sequence on keys are shared in LDS.  us, stream / block: 16 sequences behind 2k, 8 rows of 32 heads on 8 55 / 40, 16 rows 94 / 46;
-  // 8 behind 1k, 32 rows of 32 on 32 59 / 43; 32 behind 2k, 4 rows (16 columns) 70 / 70.
-  if (p->row_start && per_seq >= 32) {
-    // waves of a workgroup, workgroups that fill the CUs, least steps of a split
-    auto form = [&](int waves, long want, long least) {
-      const int cols = c->head_dim == 256 ? 128 : 32 * waves;
-      const long full = (long)c->seqs * ((per_seq + cols - 1) / cols) * c->kv_heads;
-      const long keys = p->window > 0 && !p->prefix ? std::min<long>(span, (long)p->window + cols) : span;
-      const long most = std::max(1l, std::min(want / full, 64l)), splits = std::max(1l, std::min(most, (keys + 63) / 64 / least));
-      return PagedPlan{waves, paged_tiles(columns, c->seqs, cols), (int)splits, (int)most, 0, full * splits};
-    };
-    if (c->head_dim == 256) return form(8, 256, 4);
-    // Eight waves read each block of keys from L2 and convert it once for twice the columns, two workgroups of four hide each other's
-    // waits: eight for long keys and enough columns, four where prompts are short, CUs would idle, or (heads of 64 in 16 bits) three
-    // workgroups of four fit a CU.  us, 8 / 4 waves, 32 heads on 8 of 128: 4000 rows 164 / 186, capped 205 / 242, 2 x 512 behind 7.5k in int8 194
-    // / 216, 128 behind 32k int8 108 / 126, 256 behind 8k 57 / 62; 1000 rows 38.6 / 37.8, 12 prompts of 40 - 640 60 / 54, 8 x 200 rows of 32 heads on
-    // 32 41 / 24, 64 x 64 rows 54 / 39; 512 rows 31 / 25 (64 workgroups of eight); heads of 64, 4000 rows 111 / 103, int8 130 / 149.
-    const PagedPlan wide = form(8, 256, 4), narrow = form(4, 512, 8);
-    PagedPlan plan = !(c->head_dim == 64 && c->kv_type == TI_KV_SAME) && per_seq >= 192 && span >= 2048 && wide.filled >= 192 ? wide : narrow;
-    plan.most = std::max(wide.most, narrow.most);
-    return plan;
-  }
-  if (p->window > 0 && !p->prefix) span = std::min<long>(span, (long)p->window + 16);
-  const long tiles = p->row_start ? paged_tiles(columns, c->seqs, 16) : (long)c->seqs * ((G + 15) / 16);
-  const long units = std::max(1l, tiles * c->kv_heads);
+  auto seen = [&](long rows) { return p->window > 0 && !p->prefix ? std::min(span, p->window + rows) : span; };   // by a tile of these rows
+
+  // This file's kernels.  A split has a step of each wave at least, from 17 splits on two: us, one / two, a row behind 8k of 8 kv-heads 19.6 / 16.4,
+  // 4 rows 25 / 20, one token of 5k 15.9 / 13.9 (1000 keys of 256 dims 12.8 / 14.6).  64 splits at most: a row behind 64k of one kv-head, 32 / 64 / 256
+  // splits 31 / 26 / 43, int8 128k of 8 59 / 60 / 74.
+  const long tiles = p->row_start ? paged_tiles(columns, c->seqs, 16) : (long)c->seqs * ((G + 15) / 16), units = std::max(1l, tiles * c->kv_heads);
+  const long keys = seen(16), steps = (keys + kStreamKeys - 1) / kStreamKeys, most = std::min((1024 + units - 1) / units, 64l);
+  PagedPlan stream{0, tiles, (int)std::max(1l, std::min({most, (steps + 3) / 4, std::max(16l, (steps + 7) / 8)})), (int)most, 0, 0};
   if (!p->row_start) {
-    // 256 keys are a step or two of each wave: one launch.  Workgroups a CU: 1 (32 streams of 4k - 8k, f16 of 128 dims, 1 / 2 / 3: 146 / 151 / 151 us;
-    // 48 capped of 256 dims 87 / 100 / 122), but 2 of int8 heads up to 128 dims, whose waves convert (64 of 64 dims 60 / 50 / 52, 64 x 700 37 / 32 / 39).
-    const int per_cu = c->kv_type == TI_KV_I8 && c->head_dim < 256 ? 2 : 1, deal = (int)std::max(1l, 256l * per_cu / (c->kv_heads * (long)((G + 15) / 16)));
-    return {0, tiles, 1, 1, span > 256 ? deal : 0, 0};
+    // Dealing pays where a tile's keys are many and uneven; it has every workgroup look through all lengths, and joins all.  us, splits / dealt, 8
+    // kv-heads of 128: 16 streams of 1 - 4k 39 / 38, 1 - 8k 68 / 61, 1 - 16k 121 / 102; 4 of 2k 15 / 20, 1 - 32k 71 / 59; 64 of 1 - 2k 64 / 70, 1 - 4k 117 /
+    // 107; 160 of 1 - 2k 134 / 150; 1024 of 1 - 680 373 / 654.  Of 256 dims, whose waves hold fewer loads, sooner: 16 of 500 - 1500 50 / 45, 48 of 1000 - 3000
+    // 183 / 165, 160 of 2 heads 167 / 166.  Workgroups a CU: 1 (32 streams of 4k - 8k, f16 of 128 dims, 1 / 2 / 3: 146 / 151 / 151 us; 48 capped
+    // of 256 dims 87 / 100 / 122), but 2 of int8 heads up to 128 dims, whose waves convert (64 of 64 dims 60 / 50 / 52, 64 x 700 37 / 32 / 39).
+    const int deal = (int)std::max(1l, (i8 && c->head_dim < 256 ? 512l : 256l) / (c->kv_heads * (long)((G + 15) / 16)));
+    const long bytes = 2l * c->seqs * c->kv_heads * keys * c->head_dim * (i8 ? 1 : 2), seqs = c->seqs;
+    if ((keys >= 6144 || bytes >= 192l << 20) && keys >= (c->head_dim == 256 ? std::max(512l, 20 * seqs) : std::max(2048l, 48 * seqs))) stream.deal = deal;
+    stream.most = std::max(stream.most, deal / c->seqs + 2);   // (its seqs + deal parts a head, as splits of seqs rows)
+    return stream;
   }
-  const long steps = (span + kStreamKeys - 1) / kStreamKeys, most = std::min((1024 + units - 1) / units, 256l);
-  return {0, tiles, (int)std::max(1l, std::min(most, (steps + kStreamWaves - 1) / kStreamWaves)), (int)most, 0, 0};
+  // From 32 columns a sequence on keys are shared in LDS.  us, stream / block: 16 sequences behind 2k, 8 rows of 32 heads on 8 52 / 39, 64 behind
+  // 600, 16 rows 98 / 63; 32 behind 2k, 4 rows (16 columns) 70 / 70.  But the first step of a block takes 8 us: not a few tiles of few keys (a prompt of
+  // 16 rows 7.0 / 10, 16 behind 600 12 / 15, behind 2k 17 / 17, 40 behind 600 13 / 17, behind 2k 25 / 21; 256 dims, 40 behind 600 23 / 32).
+  const bool few = units <= 256;
+  if (per_seq < 32 || (few && units * seen(per_seq / G) <= 65536)) return stream;
+  // waves of a workgroup, workgroups that fill the CUs, least steps of a split (a prompt's own keys: half of them seen)
+  auto form = [&](int waves, long want, long least) {
+    const int cols = c->head_dim == 256 ? 128 : 32 * waves;
+    const long full = (long)c->seqs * ((per_seq + cols - 1) / cols) * c->kv_heads;
+    const long n = (seen(cols) - std::min(seen(cols), per_seq / G) / 2 + 63) / 64;
+    const long most = std::max(1l, std::min(want / full, 64l)), splits = std::max(1l, std::min(most, n / least));
+    return PagedPlan{waves, paged_tiles(columns, c->seqs, cols), (int)splits, (int)std::max<long>(most, few ? stream.most : 1), 0, full * splits};
+  };
+  if (c->head_dim == 256) return form(8, 256, 4);
+  // Eight waves read each block of keys from L2 and convert it once for twice the columns, two workgroups of four hide each other's
+  // waits: eight for long keys and enough columns, four where prompts are short, CUs would idle, or (heads of 64 in 16 bits) three
+  // workgroups of four fit a CU.  us, 8 / 4 waves, 32 heads on 8 of 128: 4000 rows 164 / 186, capped 205 / 242, 2 x 512 behind 7.5k in int8 194
+  // / 216, 128 behind 32k int8 108 / 126, 256 behind 8k 57 / 62; 1000 rows 38.6 / 37.8, 12 prompts of 40 - 640 60 / 54, 8 x 200 rows of 32 heads on
+  // 32 41 / 24, 64 x 64 rows 54 / 39; 512 rows 31 / 25 (64 workgroups of eight); heads of 64, 4000 rows 111 / 103, int8 130 / 149.
+  // Least steps of four waves' splits, 8 / 4 / 2: 130 rows behind 600 34 / 24 / 22, 16 behind 600 26 / 21 / 15, 8 x 64 of 8 heads behind 2k 36 / 31 / 30.
+  const PagedPlan wide = form(8, 256, 4), narrow = form(4, 512, 2);
+  PagedPlan plan = !(c->head_dim == 64 && !i8) && per_seq >= 192 && span >= 2048 && wide.filled >= 192 ? wide : narrow;
+  plan.most = std::max(wide.most, narrow.most);
+  return plan;
 }
 
 template <int D, class T>
@@ -621,8 +632,8 @@ int launch_attn(PagedAttn a, const PagedPlan& plan, const ti_paged_cache* c, hip
 }
 
 // Parts of all rows and heads.
-static size_t parts(const ti_paged_cache* c, const ti_paged_attn_args* p, const PagedPlan& plan, int splits) {
-  return plan.deal ? (size_t)p->heads * (plan.deal + c->seqs) : splits > 1 ? (size_t)p->rows * p->heads * splits : 0;
+static size_t parts(const ti_paged_cache* c, const ti_paged_attn_args* p, const PagedPlan& plan) {
+  return plan.deal ? (size_t)p->heads * (plan.deal + c->seqs) : plan.splits > 1 ? (size_t)p->rows * p->heads * plan.splits : 0;
 }
 static size_t part_bytes(const ti_paged_cache* c, size_t n) { return n * ((size_t)c->head_dim + 2) * sizeof(float); }
 
@@ -644,7 +655,7 @@ static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_strea
   const PagedPlan plan = paged_plan(c, p);
   if (plan.tiles > (1 << 23) || (int64_t)plan.tiles * plan.splits * c->kv_heads > INT32_MAX)
     return ti_set_error(TI_ERR_ARG, "%s: %d rows of %d sequences and %d heads in a call", who, p->rows, c->seqs, p->heads);
-  const size_t n = parts(c, p, plan, plan.splits), need = part_bytes(c, n);
+  const size_t n = parts(c, p, plan), need = part_bytes(c, n);
   if (need && (!p->workspace || p->workspace_bytes < (int64_t)need))
     return ti_set_error(TI_ERR_ARG, "%s: workspace of %ld bytes, %zu needed", who, (long)(p->workspace ? p->workspace_bytes : 0), need);
   if (!p->q || !p->out) return ti_set_error(TI_ERR_ARG, "%s: null pointer", who);
@@ -669,7 +680,7 @@ extern "C" size_t ti_paged_workspace_bytes(const ti_paged_cache* c, const ti_pag
   ti_paged_attn_args any = *a;   // (of any length)
   any.max_len = any.window = 0;
   const ti::PagedPlan plan = ti::paged_plan(c, &any);
-  return ti::part_bytes(c, ti::parts(c, a, plan, plan.most));
+  return ti::part_bytes(c, (size_t)a->rows * a->heads * (plan.most > 1 ? plan.most : 0));
 }
 
 extern "C" int ti_paged_decode(const ti_paged_cache* c, const ti_paged_attn_args* a, ti_stream_t s) {

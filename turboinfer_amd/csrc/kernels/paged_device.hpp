@@ -7,7 +7,6 @@
 namespace ti {
 
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 struct PagedCache {
   void* k;

@@ -485,8 +485,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
 template <int D, int NW, class T>
 static int launch_waves(const PagedAttn& a, long tiles, bool i8, hipStream_t s) {
   const bool shaped = a.cap != 0.0f || a.slopes;
-  auto* fn = i8 ? shaped ? paged_block_kernel<D, NW, T, true, true> : paged_block_kernel<D, NW, T, true, false>
-                : shaped ? paged_block_kernel<D, NW, T, false, true> : paged_block_kernel<D, NW, T, false, false>;
+  auto* fn = shaped ? paged_block_kernel<D, NW, T, true, true> : paged_block_kernel<D, NW, T, true, false>;
+  if constexpr (D > 64 || NW == 4) {   // (heads of 64 dims in 16 bits: four waves)
+    if (!i8) fn = shaped ? paged_block_kernel<D, NW, T, false, true> : paged_block_kernel<D, NW, T, false, false>;
+  }
   // (more than 64 KiB of LDS: said once per device)
   static std::atomic<uint64_t> said[4];
   const int which = 2 * i8 + shaped;

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from paged import Cache
-from test_gpu_paged import (check_attention, test_decode, test_decode_long, test_decode_long_masks, test_decode_long_of_wide_groups,  # noqa: F401
+from test_gpu_paged import (check_append, check_attention, test_decode, test_decode_long, test_decode_long_masks, test_decode_long_of_wide_groups,  # noqa: F401
                             test_decode_of_many_sequences, test_decode_queries_of_any_size, test_decode_scores_and_masks, test_decode_sharp_and_flat_rows,
                             test_extreme_bounds, test_holes, test_int8_blocks_that_are_no_numbers, test_long_runs_of_zero_values, test_pages_that_sequences_share,
                             test_prefill, test_prefill_behind_a_long_cache, test_prefill_groups, test_prefill_many_rows, test_prefill_scores_and_masks,
@@ -40,3 +40,19 @@ def test_shared_keys_in_one_split(ti, types, dim, shaped, monkeypatch):
     lens = [n + int(x) for n, x in zip(new, rng.randint(0, 30, 32))]
     more = dict(cap=6.0, slopes=2.0 ** -rng.uniform(2, 8, 16), window=20) if shaped else {}
     check_attention(ti, Cache(ti, rng, lens, 8, dim, 16, *types), rng, 16, new, amp=2.0, **more)
+
+
+@pytest.mark.parametrize("seqs", [65, 66, 4225, 4300])
+def test_rows_of_very_many_sequences(ti, seqs, monkeypatch):
+    """Sequences of 0 to 2 rows, found in one, two and three steps; empty ones first, last and in long runs."""
+    monkeypatch.setattr(Cache, "wide", 0)
+    rng = np.random.RandomState(62)
+    new = rng.randint(0, 3, seqs)
+    new[[0, 63, 64, seqs - 1]] = 0
+    new[seqs // 3: seqs // 2] = 0
+    new = [int(x) for x in new]
+    lens = [n + int(x) for n, x in zip(new, rng.randint(0, 15, seqs))]
+    cache = Cache(ti, rng, [l - n for l, n in zip(lens, new)], 1, 64, 16, "f16", "i8", room=17)
+    cache.lens = np.asarray(lens, np.int32)
+    check_append(ti, cache, rng, new, 2, False, 32, True)
+    check_attention(ti, Cache(ti, rng, lens, 1, 64, 16, "f16", "same", room=17), rng, 2, new)

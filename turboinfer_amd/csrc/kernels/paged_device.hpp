@@ -27,15 +27,17 @@ struct PagedRows {
 __device__ __forceinline__ int paged_start(const PagedRows& r, int b) { return r.start ? r.start[b] : b; }
 
 // The last sequence whose first tile (row, ..: key(b), not falling) is at most i, by one wave: the number of b in 1 .. seqs - 1 with
-// key(b) <= i.
+// key(b) <= i.  64 keys at a time part what is left in 65: an int8 append of 4096 rows and sequences, and its read, 64
+// after 64 / so: 256 / 60 us.
 template <class Key>
 __device__ __forceinline__ int paged_find(int seqs, long i, Key key) {
   const int lane = threadIdx.x & 63;
-  int b = 0;
-  for (int b0 = 1; b0 < seqs; b0 += 64) {
-    const int n = __popcll(__builtin_amdgcn_ballot_w64(b0 + lane < seqs && key(b0 + lane) <= i));
-    b += n;
-    if (n < 64) break;
+  int b = 0, n = seqs;   // of b .. b + n - 1
+  while (n > 1) {
+    const int step = (n + 64) / 65, at = b + (lane + 1) * step;   // (64 keys between 65 parts)
+    const int below = __popcll(__builtin_amdgcn_ballot_w64((lane + 1) * step < n && key(at) <= i));
+    b += below * step;
+    n = min(step, n - below * step);
   }
   return __builtin_amdgcn_readfirstlane(b);
 }

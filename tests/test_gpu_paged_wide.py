@@ -5,13 +5,13 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from paged import Cache
-from test_gpu_paged import (check_append, check_attention, test_decode, test_decode_long, test_decode_long_masks, test_decode_long_of_wide_groups,  # noqa: F401
+from paged import HALF, Cache, from_bits, starts
+from test_gpu_paged import (MARK, check_append, check_attention, test_decode, test_decode_long, test_decode_long_masks, test_decode_long_of_wide_groups,  # noqa: F401
                             test_decode_of_many_sequences, test_decode_queries_of_any_size, test_decode_scores_and_masks, test_decode_sharp_and_flat_rows,
                             test_extreme_bounds, test_holes, test_int8_blocks_that_are_no_numbers, test_long_runs_of_zero_values, test_pages_that_sequences_share,
                             test_prefill, test_prefill_behind_a_long_cache, test_prefill_groups, test_prefill_many_rows, test_prefill_scores_and_masks,
                             test_prompts_then_steps, test_captured_prompts, test_captured_steps, test_two_streams_at_once, test_values_near_the_largest,
-                            test_values_of_many_sizes, test_values_that_are_no_numbers_in_shared_blocks, test_what_a_row_does_not_see_does_not_reach_it, types)
+                            test_values_of_many_sizes, test_values_that_are_no_numbers_in_shared_blocks, test_what_a_row_does_not_see_does_not_reach_it, types, upload)
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,22 @@ def test_rows_of_very_many_sequences(ti, seqs, monkeypatch):
     cache.lens = np.asarray(lens, np.int32)
     check_append(ti, cache, rng, new, 2, False, 32, True)
     check_attention(ti, Cache(ti, rng, lens, 1, 64, 16, "f16", "same", room=17), rng, 2, new)
+
+
+@pytest.mark.parametrize("seqs", [57, 64, 90])
+def test_read_of_narrow_rows(ti, types, seqs):
+    """Rows of 16 threads' work, of many sequences."""
+    rng = np.random.RandomState(63)
+    new = [int(x) for x in rng.randint(0, 3, seqs)]
+    lens = [n + int(x) for n, x in zip(new, rng.randint(0, 30, seqs))]
+    cache = Cache(ti, rng, lens, 1, 64, 16, *types)
+    ref, rows = cache.upload(), sum(new)
+    k, v = (upload(ti, np.full((rows + 1, 64), MARK, np.uint16)) for _ in range(2))
+    start = upload(ti, starts(new))
+    ti.check(ti.lib().ti_paged_read(ref, start.ptr, rows, k.ptr, 64, v.ptr, 64, None))
+    ti.sync()
+    for buf, name in ((k, "k"), (v, "v")):
+        got = buf.download(np.uint16, (rows + 1, 64))
+        want = np.array([cache.values(name, b, p)[0] for b, n in enumerate(new) for p in range(lens[b] - n, lens[b])])
+        assert (got[rows:] == MARK).all()
+        assert (np.abs(from_bits(got[:rows], cache.dtype) - want) <= HALF[cache.dtype] * np.abs(want) * 1.01).all()

@@ -368,10 +368,9 @@ template <int D, class T, bool I8>
 __global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 2 : 3) void paged_stream_kernel(const PagedAttn a) {
   __shared__ StreamLds<D> lds;
   const int per_seq = (a.G + 15) >> 4;
-  const int b = a.r.start ? paged_find(a.c.seqs, blockIdx.x, [&](int j) { return paged_tile0((long)a.r.start[j] * a.G, j, 16); })
-                          : (int)blockIdx.x / per_seq;
-  const PagedSeq s = paged_seq(a.c, a.r, b);
-  const long tile = a.r.start ? blockIdx.x - paged_tile0((long)s.row0 * a.G, b, 16) : (int)blockIdx.x - b * per_seq;
+  const PagedSeq s = paged_find(a.c, a.r, a.r.start ? (int)blockIdx.x : (int)blockIdx.x / per_seq,
+                                [&](int start, int j) { return paged_tile0((long)start * a.G, j, 16); });
+  const long tile = a.r.start ? blockIdx.x - paged_tile0((long)s.row0 * a.G, s.b, 16) : (int)blockIdx.x - s.b * per_seq;
   if (tile < 0 || tile * 16 >= (long)s.n * a.G) return;
   stream_tile<D, T, I8, false>(a, lds, s, tile, blockIdx.y, blockIdx.z, -1, blockIdx.z);
 }
@@ -434,7 +433,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, D == 256 && !I8 ? 1 : 2) void pa
   }
   base = uniform(base);
   for (; n > 0; n = b < a.c.seqs ? __builtin_amdgcn_readfirstlane(decode_steps(a, b)) : 0) {
-    stream_tile<D, T, I8, !(D == 256 && I8)>(a, lds, paged_seq(a.c, a.r, b), tile, kvh, (int)(max(from, base) - base), (int)min((long)n, to - base), (long)w + b);
+    stream_tile<D, T, I8, !(D == 256 && I8)>(a, lds, paged_seq(a.c, a.r, b, b, b + 1, a.c.len[b]), tile, kvh, (int)(max(from, base) - base), (int)min((long)n, to - base), (long)w + b);
     base += n;
     if (base >= to) break;
     do ++b;
@@ -508,8 +507,7 @@ template <int D, class T>
 __global__ __launch_bounds__(256) void split_join_kernel(const PagedAttn a) {
   constexpr int NT = D / 4, NH = 256 / NT, U = 8;
   const int m = blockIdx.x, d = threadIdx.x % NT * 4, head = blockIdx.y * NH + threadIdx.x / NT;
-  const int b = a.r.start ? paged_find(a.c.seqs, m, [&](int j) { return (long)a.r.start[j]; }) : m;
-  const PagedSeq s = paged_seq(a.c, a.r, b);
+  const PagedSeq s = paged_find(a.c, a.r, m, [](int start, int) { return (long)start; });
   const int p = s.pos0 + (m - s.row0);
   if (m < s.row0 || m >= s.row0 + s.n || p < 0 || p >= a.c.s.blocks * kPagedBlock || head >= a.heads) return;
   const size_t at = ((size_t)m * a.heads + head) * a.splits;

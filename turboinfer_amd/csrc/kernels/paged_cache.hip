@@ -9,8 +9,8 @@
 // and writes new and moved old tokens once.
 //
 // Bound: of many rows HBM (16-bit caches, 8000 rows of 32 heads on 8 of 128: 43 us, 4.7 TB/s; read back 32000 tokens 43.6 us, 4.8 TB/s: a large copy's
-// 4.9), int8 blocks by their chain of lookup, rows, maximum (55 us for the same rows, 3.3 TB/s; several heads a workgroup with the next one's rows
-// ahead: 59); of a step its launch (32 streams 3.3 us).
+// 4.9), int8 blocks by their chain of lookup, rows, maximum (52 us for the same rows, 3.5 TB/s; several heads a workgroup with the next one's rows
+// ahead: 4 more); of a step its launch (32 streams 3.0 us).
 #include <math.h>
 
 #include "paged_device.hpp"
@@ -83,9 +83,8 @@ template <int D, class X>
 __device__ void append_block(const AppendArgs& a, int slot, int part, float* red) {
   constexpr int CH = D / 8;
   const int tid = threadIdx.x, kvh = part >> 1, is_v = part & 1;
-  const int b = a.r.start ? paged_find(a.c.seqs, slot, [&](int j) { return paged_touch0(a.r.start[j], j); }) : slot;
-  if (b >= a.c.seqs) return;
-  const PagedSeq s = paged_seq(a.c, a.r, b);
+  const PagedSeq s = paged_find(a.c, a.r, slot, [](int start, int j) { return paged_touch0(start, j); });
+  const int b = s.b;
   const long at = a.r.start ? slot - paged_touch0(s.row0, b) : 0;
   const int pos_first = max(s.pos0, 0);
   const long blk = pos_first / kPagedBlock + at;
@@ -164,8 +163,8 @@ __global__ __launch_bounds__(2 * D) void paged_append_kernel(const AppendArgs a)
   auto fetch = [&] { return dims8(x + at / CH * D, at % CH * 8, at / CH < a.heads + a.c.s.kv_heads ? a.rot_dim : 0, a.halves); };
   Dims8 y = {};
   if (at < a.chunks) y = fetch();
-  const int b = a.r.start ? paged_find(a.c.seqs, m, [&](int j) { return (long)a.r.start[j]; }) : m;
-  const PagedSeq s = paged_seq(a.c, a.r, b);
+  const PagedSeq s = paged_find(a.c, a.r, m, [](int start, int) { return (long)start; });
+  const int b = s.b;
   const int pos = s.pos0 + (m - s.row0);
   if (m < s.row0 || m >= s.row0 + s.n || pos < 0 || pos >= a.c.s.blocks * kPagedBlock || (a.rope && pos >= a.rope_len)) return;
   const int blk = pos / kPagedBlock, entry = I8 ? 0 : a.c.table[(size_t)b * a.c.table_ld + paged_column(a.c.s, blk)];
@@ -197,9 +196,9 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const ReadArgs a) {
   constexpr int CH = D / 8;
   const int m = blockIdx.x, at = blockIdx.y * 256 + threadIdx.x, d = at % CH * 8, hh = at / CH, is_v = hh >= a.c.s.kv_heads;
   const int kvh = hh - (is_v ? a.c.s.kv_heads : 0);
-  const int b = a.r.start ? paged_find(a.c.seqs, m, [&](int j) { return (long)a.r.start[j]; }) : m;
-  if (b >= a.c.seqs || kvh >= a.c.s.kv_heads) return;
-  const PagedSeq s = paged_seq(a.c, a.r, b);
+  const PagedSeq s = paged_find(a.c, a.r, m, [](int start, int) { return (long)start; });   // (all lanes)
+  if (kvh >= a.c.s.kv_heads) return;
+  const int b = s.b;
   const int pos = s.pos0 + (m - s.row0);
   if (m < s.row0 || m >= s.row0 + s.n || pos < 0 || pos >= a.c.s.blocks * kPagedBlock) return;
   const int blk = pos / kPagedBlock;

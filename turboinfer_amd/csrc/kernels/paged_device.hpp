@@ -24,32 +24,37 @@ struct PagedRows {
   const int32_t* start;
   int rows;
 };
-__device__ __forceinline__ int paged_start(const PagedRows& r, int b) { return r.start ? r.start[b] : b; }
-
-// The last sequence whose first tile (row, ..: key(b), not falling) is at most i, by one wave: the number of b in 1 .. seqs - 1 with
-// key(b) <= i.  64 keys at a time part what is left in 65: an int8 append of 4096 rows and sequences, and its read, 64
-// after 64 / so: 256 / 60 us.
-template <class Key>
-__device__ __forceinline__ int paged_find(int seqs, long i, Key key) {
-  const int lane = threadIdx.x & 63;
-  int b = 0, n = seqs;   // of b .. b + n - 1
-  while (n > 1) {
-    const int step = (n + 64) / 65, at = b + (lane + 1) * step;   // (64 keys between 65 parts)
-    const int below = __popcll(__builtin_amdgcn_ballot_w64((lane + 1) * step < n && key(at) <= i));
-    b += below * step;
-    n = min(step, n - below * step);
-  }
-  return __builtin_amdgcn_readfirstlane(b);
-}
 
 // A sequence's rows: row0 .. row0 + n - 1 of the call, tokens pos0 ..; len: its keys, within the table.
 struct PagedSeq {
   int b, row0, n, pos0, len;
 };
-__device__ __forceinline__ PagedSeq paged_seq(const PagedCache& c, const PagedRows& r, int b) {
-  const int r0 = max(paged_start(r, b), 0), r1 = min(paged_start(r, b + 1), r.rows), n = max(r1 - r0, 0);
-  const int len = c.len[b], most = c.s.blocks * kPagedBlock;
+__device__ __forceinline__ PagedSeq paged_seq(const PagedCache& c, const PagedRows& r, int b, int from, int to, int len) {
+  const int r0 = max(from, 0), r1 = min(to, r.rows), n = max(r1 - r0, 0), most = c.s.blocks * kPagedBlock;
   return {b, r0, n, (int)max((long)len - n, (long)INT32_MIN / 2), min(max(len, 0), most)};
+}
+
+// The last sequence whose first tile (row, ..: key(row_start[b], b), not falling) is at most i, by one wave: the number of b in 1 .. seqs - 1
+// with key <= i.  Up to 64: one load of all that is asked of it, a lane each (10 rows of 4 prompts 7.3 -> 6.5 us).  More: 64 keys at a time part what is left in 65; an int8
+// append of 4096 rows and sequences, and its read, 64 after 64 / so: 256 / 60 us.  Without starts: sequence i.
+template <class Key>
+__device__ __forceinline__ PagedSeq paged_find(const PagedCache& c, const PagedRows& r, long i, Key key) {
+  if (!r.start) return paged_seq(c, r, (int)i, (int)i, (int)i + 1, c.len[i]);
+  const int lane = threadIdx.x & 63;
+  if (c.seqs <= 64) {
+    const int j = min(lane, c.seqs - 1), from = r.start[j], to = r.start[j + 1], len = c.len[j];
+    const int b = __popcll(__builtin_amdgcn_ballot_w64(lane > 0 && lane < c.seqs && key(from, j) <= i));
+    return paged_seq(c, r, b, __builtin_amdgcn_readlane(from, b), __builtin_amdgcn_readlane(to, b), __builtin_amdgcn_readlane(len, b));
+  }
+  int b = 0, n = c.seqs;   // of b .. b + n - 1
+  while (n > 1) {
+    const int step = (n + 64) / 65, at = b + (lane + 1) * step;
+    const int below = __popcll(__builtin_amdgcn_ballot_w64((lane + 1) * step < n && key(r.start[at], at) <= i));
+    b += below * step;
+    n = min(step, n - below * step);
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  return paged_seq(c, r, b, r.start[b], r.start[b + 1], c.len[b]);
 }
 
 // Values of a 16-bit type.

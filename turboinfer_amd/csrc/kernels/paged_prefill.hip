@@ -60,8 +60,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
   if (work.head < 0) return;
   const int kvh = work.head, split = work.j % a.splits;
   const long at_tile = (deal.n - 1 - work.j) / a.splits;   // (the last tiles, with the most keys, first)
-  const int b = paged_find(a.c.seqs, at_tile, [&](int j) { return paged_tile0((long)paged_start(a.r, j) * a.G, j, F::COLS); });
-  const PagedSeq s = paged_seq(a.c, a.r, b);
+  const PagedSeq s = paged_find(a.c, a.r, at_tile, [&](int start, int j) { return paged_tile0((long)start * a.G, j, F::COLS); });
+  const int b = s.b;
   const long tile = at_tile - paged_tile0((long)s.row0 * a.G, b, F::COLS);
   if (tile < 0 || tile * F::COLS >= (long)s.n * a.G) return;
   const int ci = (int)tile * F::COLS + group * 32 + c, row = ci / a.G, head = kvh * a.G + (ci - row * a.G), m = s.row0 + row, p = s.pos0 + row;

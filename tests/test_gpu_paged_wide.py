@@ -18,7 +18,7 @@ pytestmark = pytest.mark.gpu
 
 @pytest.fixture(autouse=True)
 def wide_tables(monkeypatch):
-    monkeypatch.setattr(Cache, "wide", 70000)
+    monkeypatch.setattr(Cache, "wide", 140000)
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
@@ -40,6 +40,13 @@ def test_shared_keys_in_one_split(ti, types, dim, shaped, monkeypatch):
     lens = [n + int(x) for n, x in zip(new, rng.randint(0, 30, 32))]
     more = dict(cap=6.0, slopes=2.0 ** -rng.uniform(2, 8, 16), window=20) if shaped else {}
     check_attention(ti, Cache(ti, rng, lens, 8, dim, 16, *types), rng, 16, new, amp=2.0, **more)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_shared_keys_and_windows(ti, types, dim):
+    """Windows and slopes of rows whose keys are shared, in two splits."""
+    rng = np.random.RandomState(64)
+    check_attention(ti, Cache(ti, rng, [700], 8, dim, 32, *types, holes=[(0, 9)]), rng, 16, [330], amp=2.0, window=300, slopes=2.0 ** -rng.uniform(2, 8, 16))
 
 
 @pytest.mark.parametrize("seqs", [65, 66, 4225, 4300])

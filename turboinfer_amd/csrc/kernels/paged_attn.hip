@@ -563,26 +563,34 @@ static PagedPlan paged_plan(const ti_paged_cache* c, const ti_paged_attn_args* p
   // This file's kernels.  A split has a step of each wave at least, from 17 splits on two: us, one / two, a row behind 8k of 8 kv-heads 19.6 / 16.4,
   // 4 rows 25 / 20, one token of 5k 15.9 / 13.9 (1000 keys of 256 dims 12.8 / 14.6).  64 splits at most: a row behind 64k of one kv-head, 32 / 64 / 256
   // splits 31 / 26 / 43, int8 128k of 8 59 / 60 / 74.
+  // Two workgroups a CU: us, 1024 / 768 / 512 in all, 64 streams of 700, 8 kv-heads of 128 41 / 41 / 36, of 256 86 / 86 / 77, int8 16 of 2000 of 256 39 / 41
+  // / 33, 40 of 700 of 128 21 / 19 / 20.  Few keys in one split and launch: us, one / two or more, 16 streams of 500 of 128 10.5 / 13.5, one of 256 7.6 / 9.9,
+  // of 500 9.5 / 10.0, of 768 11 - 12 / 9.8; of 64 dims, 768 8.6 / 9.8, 1024 9.8 / 9.9; of 256 dims, 256 11.5 / 12.6, 500 16 / 13.
   const long tiles = p->row_start ? paged_tiles(columns, c->seqs, 16) : (long)c->seqs * ((G + 15) / 16), units = std::max(1l, tiles * c->kv_heads);
-  const long keys = seen(16), steps = (keys + kStreamKeys - 1) / kStreamKeys, most = std::min((1024 + units - 1) / units, 64l);
-  PagedPlan stream{0, tiles, (int)std::max(1l, std::min({most, (steps + 3) / 4, std::max(16l, (steps + 7) / 8)})), (int)most, 0, 0};
+  const long keys = seen(16), steps = (keys + kStreamKeys - 1) / kStreamKeys, most = std::min((512 + units - 1) / units, 64l);
+  PagedPlan stream{0, tiles, (int)std::max(1l, std::min({keys * c->head_dim <= 65536 ? 1l : most, (steps + 3) / 4, std::max(16l, (steps + 7) / 8)})), (int)most, 0, 0};
   if (!p->row_start) {
     // Dealing pays where a tile's keys are many and uneven; it has every workgroup look through all lengths, and joins all.  us, splits / dealt, 8
     // kv-heads of 128: 16 streams of 1 - 4k 39 / 38, 1 - 8k 68 / 61, 1 - 16k 121 / 102; 4 of 2k 15 / 20, 1 - 32k 71 / 59; 64 of 1 - 2k 64 / 70, 1 - 4k 117 /
     // 107; 160 of 1 - 2k 134 / 150; 1024 of 1 - 680 373 / 654.  Of 256 dims, whose waves hold fewer loads, sooner: 16 of 500 - 1500 50 / 45, 48 of 1000 - 3000
     // 183 / 165, 160 of 2 heads 167 / 166.  Workgroups a CU: 1 (32 streams of 4k - 8k, f16 of 128 dims, 1 / 2 / 3: 146 / 151 / 151 us; 48 capped
     // of 256 dims 87 / 100 / 122), but 2 of int8 heads up to 128 dims, whose waves convert (64 of 64 dims 60 / 50 / 52, 64 x 700 37 / 32 / 39).
-    const int deal = (int)std::max(1l, (i8 && c->head_dim < 256 ? 512l : 256l) / (c->kv_heads * (long)((G + 15) / 16)));
+    // Rounded down: 52 heads, 4 / 5 workgroups each 164 / 229; from 257 heads on splits (300: 213 / 173, 250: 144 / 144).
+    const long lists = c->kv_heads * (long)((G + 15) / 16);
+    const int deal = (int)std::max(1l, (i8 && c->head_dim < 256 ? 512l : 256l) / lists);
     const long bytes = 2l * c->seqs * c->kv_heads * keys * c->head_dim * (i8 ? 1 : 2), seqs = c->seqs;
-    if ((keys >= 6144 || bytes >= 192l << 20) && keys >= (c->head_dim == 256 ? std::max(512l, 20 * seqs) : std::max(2048l, 48 * seqs))) stream.deal = deal;
+    if (lists <= 256 && (keys >= 6144 || bytes >= 192l << 20) &&
+        keys >= (c->head_dim == 256 ? std::max(512l, 20 * seqs) : std::max(2048l, 48 * seqs))) stream.deal = deal;
     stream.most = std::max(stream.most, deal / c->seqs + 2);   // (its seqs + deal parts a head, as splits of seqs rows)
     return stream;
   }
   // From 32 columns a sequence on keys are shared in LDS.  us, stream / block: 16 sequences behind 2k, 8 rows of 32 heads on 8 52 / 39, 64 behind
-  // 600, 16 rows 98 / 63; 32 behind 2k, 4 rows (16 columns) 70 / 70.  But the first step of a block takes 8 us: not a few tiles of few keys (a prompt of
-  // 16 rows 7.0 / 10, 16 behind 600 12 / 15, behind 2k 17 / 17, 40 behind 600 13 / 17, behind 2k 25 / 21; 256 dims, 40 behind 600 23 / 32).
+  // 600, 16 rows 98 / 63; 32 behind 2k, 4 rows (16 columns) 70 / 70.  But the first steps of a block take 8 us and its splits' join 4: not a few tiles
+  // of few keys.  32 heads on 8 of 128: a prompt of 16 rows 7 / 10, 64 behind 600 16 / 19, 100 behind 300 11 / 20, 600 18 / 20, 4 x 20 behind 1000 24 / 21,
+  // on 32, 100 behind 600 22 / 20; int8 100 behind 600 18 / 23, 4 x 20 behind 1000 21 / 23; of 256 dims, 40 behind 600 23 / 32, 100 behind 300 38 / 34, int8
+  // 29 / 37.
   const bool few = units <= 256;
-  if (per_seq < 32 || (few && units * seen(per_seq / G) <= 65536)) return stream;
+  if (per_seq < 32 || (few && units * seen(per_seq / G) <= (c->head_dim == 256 ? 65536 : 131072) * (i8 ? 2 : 1))) return stream;
   // waves of a workgroup, workgroups that fill the CUs, least steps of a split (a prompt's own keys: half of them seen)
   auto form = [&](int waves, long want, long least) {
     const int cols = c->head_dim == 256 ? 128 : 32 * waves;

@@ -396,7 +396,9 @@ __device__ __forceinline__ unsigned wave_scan(unsigned v) {
   }
   return v;
 }
-constexpr int kDealLeast = 2;   // steps of a run (us, 2 / 4 / 8: one stream of 2000 keys, 32 heads on 8 11.6 / 12.4 / 12.9, of 256 dims 14.6 / 16.6 / 18.1)
+// Steps of a run.  us, 1 / 2 / 4 / 8: one kv-head of 128 dims, int8, one stream of 12000 keys 19.6 / 15.3 / 14.5 / 13.8, two of 6500 16.2 / 14.3 / 13.1 / 17.3; f16, two of
+// 12000 14.3 / 14.7 / 17.1 / 16.6, of 256 dims 22.1 / 22.0 / 25.8 / 25.8.
+constexpr int kDealLeast = 2;
 __device__ __forceinline__ long deal_run(const PagedAttn& a, long all) { return max((all + a.deal - 1) / a.deal, (long)kDealLeast); }
 
 // The steps of all sequences are one list, cut into equal runs for the a.deal workgroups of a kv-head: grid (a.deal, kv-heads * tiles of 16

@@ -152,7 +152,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
   auto fetch = [&](int step, int& to, float& k, float& v) {
     const int blk = step * 4 + lane;
     to = -1;
-    if (step < s1 && blk < a.c.s.blocks) to = paged_block(a.c.s, a.c.table[(size_t)b * a.c.table_ld + paged_column(a.c.s, blk)], kvh, blk);
+    if (step + (lane >> 2) < s1 && blk < a.c.s.blocks) to = paged_block(a.c.s, a.c.table[(size_t)b * a.c.table_ld + paged_column(a.c.s, blk)], kvh, blk);
     if constexpr (I8) {
       k = v = 1.0f;
       if (to >= 0) {
@@ -166,13 +166,15 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
   constexpr bool late = D == 256 || SHAPED;
   Raw rk[F::NP], rv[F::NP];
   const int t_row = threadIdx.x / F::CH, t_ch = threadIdx.x % F::CH;
-  auto load = [&](int step) {   // this thread's chunks of a step's keys and values
+  // This thread's chunks of a step's keys and values.  (Blocks and sizes are the wave's, and said so: without, each load stands in a loop over the values
+  // that its descriptor may have; 4000 rows 165 -> 157 us, capped 203 -> 196.)
+  auto load = [&](int step) {
     const bool next = step - s0 >= 16 && ((step - s0) & 15) < 2;   // (two steps ahead: its numbers are the next ones still)
 #pragma unroll
     for (int i = 0; i < F::NP; ++i) {
       const int blk = __builtin_amdgcn_readfirstlane((i * F::RP + t_row) >> 4), l = ((step - s0) & 15) * 4 + blk;
-      const int ib = step >= s1 ? -1 : next ? __builtin_amdgcn_readlane(id_next, l) : __builtin_amdgcn_readlane(id, l);
-      const int have = ib < 0 ? 0 : max(0, min(16, s.len - 16 * (4 * step + blk))) * D * ES;
+      const int ib_now = __builtin_amdgcn_readlane(id, l), ib_next = __builtin_amdgcn_readlane(id_next, l), ib = __builtin_amdgcn_readfirstlane(next ? ib_next : ib_now);
+      const int have = __builtin_amdgcn_readfirstlane(ib < 0 ? 0 : max(0, min(16, s.len - 16 * (4 * step + blk))) * D * ES);
       const size_t off = (size_t)max(ib, 0) * (16 * D * ES);
       const int in = (((i * F::RP + t_row) & 15) * D + t_ch * 8) * ES;
       const auto krs = __builtin_amdgcn_make_buffer_rsrc((char*)a.c.k + off, 0, have, 0x00020000);

@@ -12,9 +12,9 @@
 // the registers of two waves a SIMD; they hand each other their weights through LDS, with a reference each (a whole number: moving to the larger is
 // exact).  4000 rows of 16 heads on 8: 308 -> 220 us against one wave with all of it, one a SIMD.
 //
-// Bound: one issue port for matrix products and vector instructions.  4000 rows of 32 heads on 8 of 128: 156 - 166 us (790 - 840 TFLOP/s; 16000 rows 980, a
-// library product 1218), matrix units busy 36 % of the cycles, vector instructions 47 %, LDS 33 %; with a cap 197 us, 28 % and 59 %; int8 175 - 186.  Two groups of
-// waves a phase apart (one multiplies, one weighs): 195 us, 274 with a cap.
+// Bound: one issue port for matrix products and vector instructions.  4000 rows of 32 heads on 8 of 128: 155 - 160 us (820 - 850 TFLOP/s; 16000 rows 990, a
+// library product 1218), matrix units busy 41 % of the cycles, vector instructions 48 %, LDS 37 %; with a cap 188 - 200 us, 31 % and 61 %; int8 172 - 180.  The waves
+// of a SIMD a part of a step behind each other, by four steps in LDS and barriers at two places: 159 us, 214 with a cap; a barrier every second step 163, 201.
 #include <math.h>
 
 #include <atomic>

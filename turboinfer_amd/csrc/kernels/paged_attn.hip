@@ -603,13 +603,15 @@ static PagedPlan paged_plan(const ti_paged_cache* c, const ti_paged_attn_args* p
   };
   if (c->head_dim == 256) return form(8, 256, 4);
   // Eight waves read each block of keys from L2 and convert it once for twice the columns, two workgroups of four hide each other's
-  // waits: eight for long keys and enough columns, four where prompts are short, CUs would idle, or (heads of 64 in 16 bits) three
-  // workgroups of four fit a CU.  us, 8 / 4 waves, 32 heads on 8 of 128: 4000 rows 164 / 186, capped 205 / 242, 2 x 512 behind 7.5k in int8 194
-  // / 216, 128 behind 32k int8 108 / 126, 256 behind 8k 57 / 62; 1000 rows 38.6 / 37.8, 12 prompts of 40 - 640 60 / 54, 8 x 200 rows of 32 heads on
-  // 32 41 / 24, 64 x 64 rows 54 / 39; 512 rows 31 / 25 (64 workgroups of eight); heads of 64, 4000 rows 111 / 103, int8 130 / 149.
+  // waits: eight for long keys and enough columns, four where prompts are short, CUs would idle, or (heads of 64) three workgroups of four fit
+  // a CU.  us, 8 / 4 waves, 32 heads on 8 of 128: 4000 rows 155 / 172, capped 205 / 214, 3 x 512 behind 4k 152 / 166, int8 173 / 192, 128 behind 32k int8
+  // 105 / 109, 4 x 256 behind 2k 65 / 68, 1600 behind 1500 113 / 104; 2000 rows 69 / 62, 1000 36 / 35, 8 x 200 rows of 32 heads on 32 37 / 22, 64 x 64 rows
+  // 50 / 36, 512 26 / 23 (64 workgroups of eight); heads of 64, 4000 rows 111 / 103, int8 126 / 117, 8 x 300 behind 3k 180 / 135, 2 x 512 behind 7.5k 123 / 131.
   // Least steps of four waves' splits, 8 / 4 / 2: 130 rows behind 600 34 / 24 / 22, 16 behind 600 26 / 21 / 15, 8 x 64 of 8 heads behind 2k 36 / 31 / 30.
-  const PagedPlan wide = form(8, 256, 4), narrow = form(4, 512, 2);
-  PagedPlan plan = !(c->head_dim == 64 && !i8) && per_seq >= 192 && span >= 2048 && wide.filled >= 192 ? wide : narrow;
+  const PagedPlan narrow = form(4, 512, 2);
+  if (c->head_dim == 64) return narrow;
+  const PagedPlan wide = form(8, 256, 4);
+  PagedPlan plan = per_seq >= 192 && span >= 2048 && wide.filled >= 192 ? wide : narrow;
   plan.most = std::max(wide.most, narrow.most);
   return plan;
 }

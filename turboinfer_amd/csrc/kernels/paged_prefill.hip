@@ -487,10 +487,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
 template <int D, int NW, class T>
 static int launch_waves(const PagedAttn& a, long tiles, bool i8, hipStream_t s) {
   const bool shaped = a.cap != 0.0f || a.slopes;
-  auto* fn = shaped ? paged_block_kernel<D, NW, T, true, true> : paged_block_kernel<D, NW, T, true, false>;
-  if constexpr (D > 64 || NW == 4) {   // (heads of 64 dims in 16 bits: four waves)
-    if (!i8) fn = shaped ? paged_block_kernel<D, NW, T, false, true> : paged_block_kernel<D, NW, T, false, false>;
-  }
+  auto* fn = i8 ? shaped ? paged_block_kernel<D, NW, T, true, true> : paged_block_kernel<D, NW, T, true, false>
+                : shaped ? paged_block_kernel<D, NW, T, false, true> : paged_block_kernel<D, NW, T, false, false>;
   // (more than 64 KiB of LDS: said once per device)
   static std::atomic<uint64_t> said[4];
   const int which = 2 * i8 + shaped;
@@ -507,9 +505,13 @@ static int launch_waves(const PagedAttn& a, long tiles, bool i8, hipStream_t s) 
 }
 template <int D, class T>
 static int launch(const PagedAttn& a, int waves, long tiles, bool i8, hipStream_t s) {
-  if constexpr (D < 256)
-    if (waves == 4) return launch_waves<D, 4, T>(a, tiles, i8, s);
-  return launch_waves<D, 8, T>(a, tiles, i8, s);
+  if constexpr (D == 64) {
+    return launch_waves<D, 4, T>(a, tiles, i8, s);
+  } else {
+    if constexpr (D == 128)
+      if (waves == 4) return launch_waves<D, 4, T>(a, tiles, i8, s);
+    return launch_waves<D, 8, T>(a, tiles, i8, s);
+  }
 }
 
 int paged_block_run(const PagedAttn& a, const ti_paged_cache* c, int waves, long tiles, hipStream_t s) {

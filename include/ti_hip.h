@@ -456,7 +456,8 @@ int ti_paged_read(const ti_paged_cache* c, const int32_t* row_start, int rows, v
  * kv_heads).  Row at token p scores key j
  *   s = scale * (q . k_j);  softcap > 0: s = softcap * tanh(s / softcap);  slopes: s += slopes[h] * (j - p)
  * and sees it where first[row] <= j < len, j <= p or j < prefix[sequence], and window = 0 or j > p - window.  out = sum of softmax(s)
- * v; a row that sees no key: 0.  |scale| <= 1e30, softcap 0 or 1e-20 .. 1e30.  What a row does not see does not reach it, infinities and NaN among it.  fp32 scores, sums and
+ * v; a row that sees no key: 0.  |scale| <= 1e30, softcap 0 or 1e-20 .. 1e30 (a capped score is off by
+ * 2^-20 of itself at most, by caps of 1 / 16 to 64 by 2^-22 of the cap).  What a row does not see does not reach it, infinities and NaN among it.  fp32 scores, sums and
  * weights; weights are rounded to 16 bits (TI_KV_I8: fp16) for their products with the values.
  * ti_paged_decode: one row a sequence (rows = seqs, row_start NULL).  ti_paged_prefill: any rows.
  * max_len: about the longest sequence (0: the table's size); it shapes the work only, as ti_attn_decode's splits do.

@@ -62,7 +62,7 @@ struct StreamLds {
 
 // One tile of a sequence over some of its keys: steps u0 .. u1 - 1 of 32, counted from the tile's first (u1 < 0: split u0's part of all).
 // Sums go to part `at` of a row's head, or (a.splits 1) the result to `out`.
-template <int D, class T, bool I8, bool AHEAD>   // AHEAD: the next step's loads stand in front of a step's products
+template <int D, class T, bool I8, bool FAR, bool AHEAD>   // FAR: a cap that is not near; AHEAD: the next step's loads stand in front of a step's products
 __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_lds, const PagedSeq& s, long tile, int kvh, int u0, int u1, long slot) {
   typedef typename PagedMat<T, I8>::M M;
   typedef typename PagedMat<T, I8>::V8 V8;
@@ -93,7 +93,7 @@ __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_
 
   // queries: 16-bit keys' step c: dims 32 c + 8 g ..; int8: dims 64 (c / 2) + 16 g + 8 (c & 1) ..
   V8 qf[NK];
-  float f = a.f;
+  float f = a.f, fx = a.fx;
   {
     const T* qr = (const T*)a.q + (size_t)m * a.ldq + (size_t)head * D;
     u16x8 raw[NK];
@@ -116,7 +116,10 @@ __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_
       const int ex = (int)(top >> 7) - 127;   // (0, subnormal, infinite: as they are)
       const bool scaled = top != 0 && top != 0x7f80u;
       const float up = scaled ? ldexpf(1.0f, -ex) : 1.0f;
-      if (scaled) f = ldexpf(f, ex);
+      if (scaled) {
+        f = ldexpf(f, ex);
+        fx = ldexpf(fx, ex);
+      }
 #pragma unroll
       for (int c = 0; c < NK; ++c)
 #pragma unroll
@@ -186,6 +189,17 @@ __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_
         const int id0 = __builtin_amdgcn_readlane(id, 2 * i), id1 = __builtin_amdgcn_readlane(id, 2 * i + 1);
         const bool ragged = key0 < lo_all || key0 + kStreamKeys - 1 > hi_all || (id0 | id1) < 0;
         float vl[2] = {0.0f, 0.0f}, vi[2] = {1.0f, 1.0f};
+        if constexpr (FAR) {
+          float fk[2] = {f, f}, fxk[2] = {fx, fx};
+          if constexpr (I8)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const float sk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), 2 * i + t));
+              fk[t] *= sk;
+              fxk[t] *= sk;
+            }
+          paged_cap<4>(a.cap, sc, fk, fxk);
+        }
         float mx = -INFINITY;
         uint32_t see = 255;
         if (ragged) {
@@ -202,14 +216,14 @@ __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          float ft = f;
+          float ft = FAR ? 1.0f : f;
           if constexpr (I8) {
-            ft *= __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), 2 * i + t));
+            if constexpr (!FAR) ft *= __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), 2 * i + t));
             const float sv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), 2 * i + t));
             vl[t] = __builtin_amdgcn_logf(sv);
             vi[t] = ragged && !(see >> 4 * t & 15) ? 0.0f : __builtin_amdgcn_rcpf(sv) * kPagedUnit;   // (0 of a block, whose scale may be NaN)
           }
-          if (a.cap != 0.0f) {
+          if (!FAR && a.cap != 0.0f) {
             asm volatile("" : "+v"(ft));
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[t][e] = paged_capped(sc[t][e], ft);
@@ -364,7 +378,7 @@ __device__ __forceinline__ void stream_tile(const PagedAttn& a, StreamLds<D>& x_
 
 // Grid (tiles, kv-heads, splits).  Steps are few: more waves a CU instead of the next step's loads in flight (us, 46 x 30 - 84 keys, 32 heads on 32: dims of
 // 128 18.6 -> 13.8, 256 52.6 -> 34.0, in int8 45.8 -> 25.0; 64 x 145 - 200 of 128 dims 42.6 -> 38.1).
-template <int D, class T, bool I8>
+template <int D, class T, bool I8, bool FAR>
 __global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 2 : 3) void paged_stream_kernel(const PagedAttn a) {
   __shared__ StreamLds<D> lds;
   const int per_seq = (a.G + 15) >> 4;
@@ -372,7 +386,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, D == 256 ? 2 : 3) void paged_str
                                 [&](int start, int j) { return paged_tile0((long)start * a.G, j, 16); });
   const long tile = a.r.start ? blockIdx.x - paged_tile0((long)s.row0 * a.G, s.b, 16) : (int)blockIdx.x - s.b * per_seq;
   if (tile < 0 || tile * 16 >= (long)s.n * a.G) return;
-  stream_tile<D, T, I8, false>(a, lds, s, tile, blockIdx.y, blockIdx.z, -1, blockIdx.z);
+  stream_tile<D, T, I8, FAR, false>(a, lds, s, tile, blockIdx.y, blockIdx.z, -1, blockIdx.z);
 }
 
 // Single tokens: steps of 32 keys that sequence b's row sees.
@@ -404,7 +418,7 @@ __device__ __forceinline__ long deal_run(const PagedAttn& a, long all) { return 
 // The steps of all sequences are one list, cut into equal runs for the a.deal workgroups of a kv-head: grid (a.deal, kv-heads * tiles of 16
 // query heads).  Part w + b of a head is workgroup w's of sequence b: each differs from the one in front by 1 in
 // w or more in b.
-template <int D, class T, bool I8>
+template <int D, class T, bool I8, bool FAR>
 __global__ __launch_bounds__(64 * kStreamWaves, D == 256 && !I8 ? 1 : 2) void paged_deal_kernel(const PagedAttn a) {
   __shared__ StreamLds<D> lds;
   const int lane = threadIdx.x & 63, w = blockIdx.x, per_seq = (a.G + 15) >> 4, kvh = blockIdx.y / per_seq, tile = blockIdx.y - kvh * per_seq;
@@ -435,7 +449,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, D == 256 && !I8 ? 1 : 2) void pa
   }
   base = uniform(base);
   for (; n > 0; n = b < a.c.seqs ? __builtin_amdgcn_readfirstlane(decode_steps(a, b)) : 0) {
-    stream_tile<D, T, I8, !(D == 256 && I8)>(a, lds, paged_seq(a.c, a.r, b, b, b + 1, a.c.len[b]), tile, kvh, (int)(max(from, base) - base), (int)min((long)n, to - base), (long)w + b);
+    stream_tile<D, T, I8, FAR, !(D == 256 && I8)>(a, lds, paged_seq(a.c, a.r, b, b, b + 1, a.c.len[b]), tile, kvh, (int)(max(from, base) - base), (int)min((long)n, to - base), (long)w + b);
     base += n;
     if (base >= to) break;
     do ++b;
@@ -622,11 +636,15 @@ int launch_attn(PagedAttn a, const PagedPlan& plan, const ti_paged_cache* c, hip
   if (plan.waves) {
     if (const int rc = paged_block_run(a, c, plan.waves, plan.tiles, s)) return rc;
   } else if (plan.deal) {
-    hipLaunchKernelGGL((i8 ? paged_deal_kernel<D, T, true> : paged_deal_kernel<D, T, false>), dim3(plan.deal, c->kv_heads * ((a.G + 15) / 16)),
+    auto* fn = a.far ? i8 ? paged_deal_kernel<D, T, true, true> : paged_deal_kernel<D, T, false, true>
+                     : i8 ? paged_deal_kernel<D, T, true, false> : paged_deal_kernel<D, T, false, false>;
+    hipLaunchKernelGGL(fn, dim3(plan.deal, c->kv_heads * ((a.G + 15) / 16)),
                        dim3(64 * kStreamWaves), 0, s, a);
     TI_LAUNCH_CHECK("paged_deal_kernel");
   } else {
-    hipLaunchKernelGGL((i8 ? paged_stream_kernel<D, T, true> : paged_stream_kernel<D, T, false>), dim3((unsigned)plan.tiles, c->kv_heads, plan.splits),
+    auto* fn = a.far ? i8 ? paged_stream_kernel<D, T, true, true> : paged_stream_kernel<D, T, false, true>
+                     : i8 ? paged_stream_kernel<D, T, true, false> : paged_stream_kernel<D, T, false, false>;
+    hipLaunchKernelGGL(fn, dim3((unsigned)plan.tiles, c->kv_heads, plan.splits),
                        dim3(64 * kStreamWaves), 0, s, a);
     TI_LAUNCH_CHECK("paged_stream_kernel");
   }
@@ -677,9 +695,12 @@ static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_strea
   if (p->rows == 0) return TI_OK;
   float* ws = (float*)p->workspace;
   const float cap = p->softcap;
-  const PagedAttn a = {ti_paged_form(c), {p->row_start, p->rows}, p->q, p->out, p->slopes, p->first, p->prefix, n ? ws : nullptr,
-                       n ? ws + n * c->head_dim : nullptr, p->heads, p->heads / c->kv_heads, p->ldq, p->ldo, p->window, plan.splits, plan.deal,
-                       c->kv_type == TI_KV_I8 ? kPagedUnit : 1.0f, cap > 0.0f ? 2.0f * p->scale * kPagedLog2e / cap : p->scale * kPagedLog2e, 2.0f * cap * kPagedLog2e};
+  const bool near = cap > 0.0f && paged_cap_near(cap, p->scale), far = cap > 0.0f && !near;
+  PagedAttn a = {ti_paged_form(c), {p->row_start, p->rows}, p->q, p->out, p->slopes, p->first, p->prefix, n ? ws : nullptr,
+                 n ? ws + n * c->head_dim : nullptr, p->heads, p->heads / c->kv_heads, p->ldq, p->ldo, p->window, plan.splits, plan.deal,
+                 c->kv_type == TI_KV_I8 ? kPagedUnit : 1.0f, near ? 2.0f * p->scale * kPagedLog2e / cap : p->scale * kPagedLog2e,
+                 near ? 2.0f * cap * kPagedLog2e : cap * kPagedLog2e, 0.0f, far};
+  if (far) a.fx = (float)std::clamp((double)p->scale / cap, -(double)kPagedMost, (double)kPagedMost);
   return TI_PAGED_FORM(c, launch_attn, a, plan, c, (hipStream_t)stream_);
 }
 

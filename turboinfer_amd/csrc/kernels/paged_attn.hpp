@@ -20,7 +20,9 @@ struct PagedAttn {
   float* part_ml;   // [..][2]: reference, denominator
   int heads, G, ldq, ldo, window, splits, deal;
   float unit;       // of the denominators: int8 kPagedUnit, else 1
-  float f, cap;     // weights are 2^(f s), or with a cap 2^(cap paged_capped(s, f))
+  float f, cap;     // weights are 2^(f s), or with a cap 2^(cap paged_capped(s, f)); caps that are not near: 2^(cap tanh(fx s)) (paged_cap)
+  float fx;
+  int far;          // a cap that is not near
 };
 
 constexpr float kPagedLog2e = 1.44269504088896341f;
@@ -57,8 +59,53 @@ __device__ __forceinline__ uint32_t i8_of(uint32_t x) {
 }
 
 // A score under a cap c, c tanh(x) = c - 2 c / (e^2x + 1): what 2 c log2 e (PagedAttn::cap) is multiplied with to an exponent of 2, without the
-// first term, which all keys have.  f: 2 scale log2 e / c (int8: times the keys' scale).
+// first term, which all keys have.  f: 2 scale log2 e / c (int8: times the keys' scale).  Its error goes with the cap, 2^-22 of it.
 __device__ __forceinline__ float paged_capped(float s, float f) { return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s * f)); }
+// So it serves caps of which that is less than a weight's rounding to 16 bits (2^-16 at 64), and with which f stays finite and normal.
+static inline bool paged_cap_near(float cap, float scale) { return cap >= 0x1p-4f && cap <= 64.0f && fabsf(scale) >= 0x1p-100f; }
+
+// Any other cap: exponents of 2 in place of the scores, C tanh(x), C = c log2 e (PagedAttn::cap), with errors that go with the score.
+//   |x| <= 1/2: f s P(x^2), f = scale log2 e, P = tanh(x) / x within 2^-25 (minimax polynomial of 4 terms);
+//   else: C - 2 C / (e^2x + 1), where the score is at least 0.46 of the cap.
+// Where all of a wave's are small, and they are where a cap is meant to do nothing, only the first is computed.  In kernels of their own: us, 4000 rows of
+// 32 heads on 8 of 128, cap 1000, this / paged_capped 194 / 188, int8 223 / 210, heads of 64 164 / 135; with this by a ballot in the kernels of near caps
+// those took more registers, cap 30 197 instead of 189, slopes alone 180 instead of 174, int8 of 64 dims 205 instead of 176.
+// sc: KT vectors of scores, E of them a block of keys; f, fx (x = fx s) by blocks.
+constexpr float kPagedMost = 1e38f;   // of |fx|, so that 2 log2 e times it, times a score of 0, is 0
+__device__ __forceinline__ float paged_tanh_ratio(float x) {
+  const float u = x * x;
+  return fmaf(u, fmaf(u, fmaf(u, fmaf(u, 0x1.1a7c0ep-6f, -0x1.b28c76p-5f), 0x1.10e9fcp-3f), -0x1.5554d6p-2f), 1.0f);
+}
+template <int E, int KT, class V>
+__device__ __forceinline__ void paged_cap(float cap, V (&sc)[KT], const float* f, const float* fx) {
+  constexpr int N = sizeof(V) / sizeof(float), B = N / E;
+  float top = 0.0f, m[KT * B];
+#pragma unroll
+  for (int b = 0; b < KT * B; ++b) m[b] = fx[b] > kPagedMost ? kPagedMost : fx[b] < -kPagedMost ? -kPagedMost : fx[b];   // (NaN stays)
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(sc[t][i] * m[t * B + i / E]));
+#pragma unroll
+  for (int b = 0; b < KT * B; ++b) asm volatile("" : "+v"(m[b]));   // (the products again, not 32 of them kept)
+  if (__builtin_amdgcn_ballot_w64(top > 0.5f) == 0) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < N; ++i) sc[t][i] *= f[t * B + i / E] * paged_tanh_ratio(sc[t][i] * m[t * B + i / E]);
+  } else {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int b = t * B + i / E;
+        const float x = sc[t][i] * m[b], big = fmaf(2.0f * cap, paged_capped(x, 2.0f * kPagedLog2e), cap);
+        float y = fabsf(x) > 0.5f ? big : sc[t][i] * f[b] * paged_tanh_ratio(x);
+        asm volatile("" : "+v"(y), "+v"(m[b]));   // (a few at a time: registers)
+        sc[t][i] = y;
+      }
+  }
+}
 
 // Keys that a row at token p sees: [lo, hi].
 struct PagedSpan {

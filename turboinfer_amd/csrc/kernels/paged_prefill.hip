@@ -43,12 +43,12 @@ __device__ __forceinline__ int key_at(int r, int c) { return r * (2 * D) + ((c ^
 template <int D>
 __device__ __forceinline__ int value_at(int r, int c) { return r * (2 * D) + ((((c >> 1) ^ (D == 64 ? (r >> 1) & 3 : r & 7)) << 5) | (c & 1) << 4); }
 
-template <int D, int NW, class T, bool I8, bool SHAPED>   // SHAPED: scores with a cap or slopes
-__global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_kernel(const PagedAttn a, const XcdDeal deal) {
+template <int D, int NW, class T, bool I8, int SHAPE>   // SHAPE: scores with 1: a near cap or slopes; 2: any other cap, slopes
+__global__ __launch_bounds__(64 * NW, D == 64 && !I8 && SHAPE < 2 ? 3 : 2) void paged_block_kernel(const PagedAttn a, const XcdDeal deal) {
   typedef BlockForm<D, NW> F;
   typedef typename PagedMat<T, I8>::M M;
   typedef typename PagedMat<T, I8>::V8 V8;
-  constexpr bool PAIR = F::PAIR;
+  constexpr bool PAIR = F::PAIR, SHAPED = SHAPE > 0, FAR = SHAPE == 2;
   constexpr int NK = D / 16, NV = D / (PAIR ? 64 : 32), KT = PAIR ? 1 : 2, ES = I8 ? 1 : 2;   // this wave's: tiles of dimensions, of keys
   typedef std::conditional_t<I8, u32x2, u32x4> Raw;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
   if (threadIdx.x == 0) odd = 0;
 
   V8 qf[NK];
-  float f = a.f;
+  float f = a.f, fx = fabsf(a.fx);
   {
     const T* qr = (const T*)a.q + (size_t)m * a.ldq + (size_t)head * D;
     u16x8 raw[NK];
@@ -114,7 +114,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
       const int ex = (int)(top >> 7) - 127;
       const bool scaled = top != 0 && top != 0x7f80u;
       const float up = scaled ? ldexpf(1.0f, -ex) : 1.0f;
-      if (scaled) f = ldexpf(f, ex);
+      if (scaled) {
+        f = ldexpf(f, ex);
+        fx = ldexpf(fx, ex);
+      }
 #pragma unroll
       for (int k = 0; k < NK; ++k)
 #pragma unroll
@@ -296,7 +299,14 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
     }
     // exponents of 2: mul[block] s + add[block]
     float mul[2 * KT], add[2 * KT], mx = -INFINITY;
-    if (SHAPED && a.cap != 0.0f) {
+    if constexpr (FAR) {
+      float fxk[2 * KT];
+#pragma unroll
+      for (int t = 0; t < 2 * KT; ++t) fxk[t] = I8 ? fx * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), l0 + t)) : fx;
+      paged_cap<8>(a.cap, sc, fk, fxk);
+#pragma unroll
+      for (int t = 0; t < 2 * KT; ++t) fk[t] = 1.0f;
+    } else if (SHAPED && a.cap != 0.0f) {
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -486,12 +496,14 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 ? 3 : 2) void paged_block_k
 
 template <int D, int NW, class T>
 static int launch_waves(const PagedAttn& a, long tiles, bool i8, hipStream_t s) {
-  const bool shaped = a.cap != 0.0f || a.slopes;
-  auto* fn = i8 ? shaped ? paged_block_kernel<D, NW, T, true, true> : paged_block_kernel<D, NW, T, true, false>
-                : shaped ? paged_block_kernel<D, NW, T, false, true> : paged_block_kernel<D, NW, T, false, false>;
+  const int shape = a.far ? 2 : a.cap != 0.0f || a.slopes ? 1 : 0;
+  static constexpr decltype(&paged_block_kernel<D, NW, T, true, 2>) kernels[2][3] = {
+      {paged_block_kernel<D, NW, T, false, 0>, paged_block_kernel<D, NW, T, false, 1>, paged_block_kernel<D, NW, T, false, 2>},
+      {paged_block_kernel<D, NW, T, true, 0>, paged_block_kernel<D, NW, T, true, 1>, paged_block_kernel<D, NW, T, true, 2>}};
+  auto* fn = kernels[i8][shape];
   // (more than 64 KiB of LDS: said once per device)
-  static std::atomic<uint64_t> said[4];
-  const int which = 2 * i8 + shaped;
+  static std::atomic<uint64_t> said[6];
+  const int which = 3 * i8 + shape;
   int dev = 0;
   TI_HIP_CHECK(hipGetDevice(&dev), "hipGetDevice");
   if (!(said[which].load(std::memory_order_relaxed) >> (dev & 63) & 1)) {

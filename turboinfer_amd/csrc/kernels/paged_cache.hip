@@ -89,6 +89,7 @@ __device__ void append_block(const AppendArgs& a, int slot, int part, float* red
   const int pos_first = max(s.pos0, 0);
   const long blk = pos_first / kPagedBlock + at;
   if (s.n == 0 || at < 0 || blk * kPagedBlock >= (long)s.pos0 + s.n || blk >= a.c.s.blocks) return;
+  if (a.rope && max(s.pos0, (int)blk * kPagedBlock) >= a.rope_len) return;   // (no fresh row: neither tokens nor scale change)
   const int id = paged_block(a.c.s, a.c.table[(size_t)b * a.c.table_ld + paged_column(a.c.s, (int)blk)], kvh, (int)blk);
   if (id < 0) return;
   const int tok = tid / CH, d = tid % CH * 8, pos = (int)blk * kPagedBlock + tok;

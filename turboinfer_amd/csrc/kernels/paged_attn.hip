@@ -400,7 +400,7 @@ __device__ __forceinline__ int decode_steps(const PagedAttn& a, int b) {
 __device__ __forceinline__ long uniform(long v) {
   return (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
 }
-// Sum over this lane and those in front of it.  (64 sequences of at most 2^26 steps: 32 bits unsigned.)
+// Sum over this lane and those in front of it.  (64 sequences of less than 2^26 steps, as paged_plan sees to: 32 bits unsigned.)
 __device__ __forceinline__ unsigned wave_scan(unsigned v) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -594,8 +594,10 @@ static PagedPlan paged_plan(const ti_paged_cache* c, const ti_paged_attn_args* p
     // Rounded down: 52 heads, 4 / 5 workgroups each 164 / 229; from 257 heads on splits (300: 213 / 173, 250: 144 / 144).
     const long lists = c->kv_heads * (long)((G + 15) / 16);
     const int deal = (int)std::max(1l, (i8 && c->head_dim < 256 ? 512l : 256l) / lists);
+    // (64 sequences of the longest table's 2^26 steps would pass the runs' sums: wave_scan)
+    const bool sums = (long)c->table_ld * c->page <= (1l << 31) - kStreamKeys;
     const long bytes = 2l * c->seqs * c->kv_heads * keys * c->head_dim * (i8 ? 1 : 2), seqs = c->seqs;
-    if (lists <= 256 && (keys >= 6144 || bytes >= 192l << 20) &&
+    if (sums && lists <= 256 && (keys >= 6144 || bytes >= 192l << 20) &&
         keys >= (c->head_dim == 256 ? std::max(512l, 20 * seqs) : std::max(2048l, 48 * seqs))) stream.deal = deal;
     stream.most = std::max(stream.most, deal / c->seqs + 2);   // (its seqs + deal parts a head, as splits of seqs rows)
     return stream;

@@ -30,6 +30,7 @@ __device__ __forceinline__ f32x16 pmma32(f16x8 a, f16x8 b, f32x16 c) { return __
 __device__ __forceinline__ f32x16 pmma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 constexpr int kBlockKeys = 64;
+constexpr float kPagedLeast = 0x1p-149f;
 template <int D, int NW>   // NW: waves
 struct BlockForm {
   static constexpr bool PAIR = D == 256;   // two waves a column: each half of a step's keys, and of the dimensions
@@ -331,9 +332,9 @@ __global__ __launch_bounds__(64 * NW, D == 64 && !I8 && SHAPE < 2 ? 3 : 2) void 
       }
     } else {
 #pragma unroll
-      for (int t = 0; t < 2 * KT; ++t) {   // (what is masked stays -inf: a factor > 0, and none of a block that is not seen)
+      for (int t = 0; t < 2 * KT; ++t) {   // (what is masked stays -inf: a factor > 0, the least there is, which makes nothing of any score; none of a block that is not seen)
         const bool none = I8 && ragged && !(see[t >> 1] >> 8 * (t & 1) & 255);
-        mul[t] = none ? 1.0f : fk[t] < 0x1p-120f ? 0x1p-120f : fk[t];
+        mul[t] = none ? 1.0f : fk[t] < kPagedLeast ? kPagedLeast : fk[t];
         add[t] = none ? 0.0f : vl[t];
       }
     }

@@ -479,6 +479,9 @@ typedef struct ti_paged_attn_args {
 size_t ti_paged_workspace_bytes(const ti_paged_cache* c, const ti_paged_attn_args* a);
 int ti_paged_decode(const ti_paged_cache* c, const ti_paged_attn_args* a, ti_stream_t s);
 int ti_paged_prefill(const ti_paged_cache* c, const ti_paged_attn_args* a, ti_stream_t s);
+/* What ti_paged_decode and ti_paged_prefill launch for these sizes, e.g. "paged_block_kernel<128,8,16 bits,plain>, splits 4"
+ * (bench / profile labels, tests). */
+int ti_paged_kernel_name(const ti_paged_cache* c, const ti_paged_attn_args* a, char* buf, int len);
 /* sizeof(ti_paged_cache), ti_paged_append_args, ti_paged_attn_args (which = 0, 1, 2): a binding checks its mirrors against them. */
 int ti_paged_struct_bytes(int which);
 

@@ -174,7 +174,7 @@ EXPORTED = [
     "ti_gqa_prep", "ti_gqa_block_elems", "ti_gqa_decode", "ti_gqa_prefill", "ti_gqa_splits", "ti_recurrent_prepare", "ti_conv",
     "ti_ssd_step", "ti_ssd_scan", "ti_ssd_norm", "ti_lru_scan", "ti_lru_step", "ti_lru_step_max_block", "ti_stack_kpad", "ti_stack_weight_bytes", "ti_stack_pack",
     "ti_stack_convert", "ti_stack_fill", "ti_dense", "ti_dense_tile", "ti_dense_args_bytes", "ti_rownorm", "ti_rownorm_routes", "ti_route", "ti_route_max_tiles",
-    "ti_paged_append", "ti_paged_read", "ti_paged_workspace_bytes", "ti_paged_decode", "ti_paged_prefill", "ti_paged_struct_bytes",
+    "ti_paged_append", "ti_paged_read", "ti_paged_workspace_bytes", "ti_paged_decode", "ti_paged_prefill", "ti_paged_kernel_name", "ti_paged_struct_bytes",
     "ti_latent_prep", "ti_latent_prepare", "ti_latent_attn_decode", "ti_latent_attn_splits", "ti_latent_attn_prefill", "ti_latent_attn_out",
 ]
 
@@ -247,6 +247,8 @@ def lib() -> C.CDLL:
             L.ti_paged_workspace_bytes.argtypes = [cache, attn]
             L.ti_paged_workspace_bytes.restype = sz
             L.ti_paged_decode.argtypes = L.ti_paged_prefill.argtypes = [cache, attn, vp]
+        if hasattr(L, "ti_paged_kernel_name"):
+            L.ti_paged_kernel_name.argtypes = [cache, attn, C.c_char_p, i32]
         if hasattr(L, "ti_sample_device"):
             L.ti_sample_device.argtypes = [vp, i32, i32, i32, f32, i32, f32, vp, vp, vp, vp]
         if hasattr(L, "ti_sample_device_ws"):
@@ -417,6 +419,13 @@ def hbm_calibrate(nbytes: int = 1 << 30, reps: int = 5) -> tuple[float, float]:
 def gemm_kernel_name(bits: int, x_kind: int, M: int, N: int, K: int) -> str:
     buf = C.create_string_buffer(64)
     check(lib().ti_gemm_kernel_name(bits, x_kind, M, N, K, buf, 64))
+    return buf.value.decode()
+
+
+def paged_kernel_name(cache: PagedCache, args: PagedAttnArgs) -> str:
+    """What ti_paged_decode or ti_paged_prefill launches for a call of these sizes (bench / profile labels)."""
+    buf = C.create_string_buffer(96)
+    check(lib().ti_paged_kernel_name(C.byref(cache), C.byref(args), buf, 96))
     return buf.value.decode()
 
 

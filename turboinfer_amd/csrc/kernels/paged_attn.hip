@@ -22,6 +22,7 @@
 // Bound: HBM.  us and TB/s: 32 streams of 4k - 8k, 32 heads on 8 of 128, int8 87 / 4.6, f16 146 / 5.5; one of 128k int8 59 / 4.6; without any arithmetic 82, 145, 57.
 // Loads of the next step stand in front of a step's products; loading keys behind theirs, values behind theirs needs no more registers, but int8 took 99.
 #include <math.h>
+#include <stdio.h>
 
 #include "paged_attn.hpp"
 
@@ -680,6 +681,8 @@ static int check_attn(const ti_paged_cache* c, const ti_paged_attn_args* p, cons
   return TI_OK;
 }
 
+static bool far_cap(const ti_paged_attn_args* p) { return p->softcap > 0.0f && !paged_cap_near(p->softcap, p->scale); }
+
 static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_stream_t stream_, const char* who) {
   if (const int rc = check_attn(c, p, who)) return rc;
   const PagedPlan plan = paged_plan(c, p);
@@ -697,7 +700,7 @@ static int attend(const ti_paged_cache* c, const ti_paged_attn_args* p, ti_strea
   if (p->rows == 0) return TI_OK;
   float* ws = (float*)p->workspace;
   const float cap = p->softcap;
-  const bool near = cap > 0.0f && paged_cap_near(cap, p->scale), far = cap > 0.0f && !near;
+  const bool far = far_cap(p), near = cap > 0.0f && !far;
   PagedAttn a = {ti_paged_form(c), {p->row_start, p->rows}, p->q, p->out, p->slopes, p->first, p->prefix, n ? ws : nullptr,
                  n ? ws + n * c->head_dim : nullptr, p->heads, p->heads / c->kv_heads, p->ldq, p->ldo, p->window, plan.splits, plan.deal,
                  c->kv_type == TI_KV_I8 ? kPagedUnit : 1.0f, near ? 2.0f * p->scale * kPagedLog2e / cap : p->scale * kPagedLog2e,
@@ -714,6 +717,20 @@ extern "C" size_t ti_paged_workspace_bytes(const ti_paged_cache* c, const ti_pag
   any.max_len = any.window = 0;
   const ti::PagedPlan plan = ti::paged_plan(c, &any);
   return ti::part_bytes(c, (size_t)a->rows * a->heads * (plan.most > 1 ? plan.most : 0));
+}
+
+extern "C" int ti_paged_kernel_name(const ti_paged_cache* c, const ti_paged_attn_args* a, char* buf, int len) {
+  if (!buf || len < 1) return ti_set_error(TI_ERR_ARG, "ti_paged_kernel_name: null buffer");
+  if (const int rc = ti::check_attn(c, a, "ti_paged_kernel_name")) return rc;
+  const ti::PagedPlan plan = ti::paged_plan(c, a);
+  const char *kv = c->kv_type == TI_KV_I8 ? "int8" : "16 bits", *cap = ti::far_cap(a) ? "far cap" : a->softcap != 0.0f || a->slopes ? "shaped" : "plain";
+  if (plan.waves)
+    snprintf(buf, (size_t)len, "paged_block_kernel<%d,%d,%s,%s>, splits %d", c->head_dim, plan.waves, kv, cap, plan.splits);
+  else if (plan.deal)
+    snprintf(buf, (size_t)len, "paged_deal_kernel<%d,%s,%s>, runs %d", c->head_dim, kv, cap, plan.deal);
+  else
+    snprintf(buf, (size_t)len, "paged_stream_kernel<%d,%s,%s>, splits %d", c->head_dim, kv, cap, plan.splits);
+  return TI_OK;
 }
 
 extern "C" int ti_paged_decode(const ti_paged_cache* c, const ti_paged_attn_args* a, ti_stream_t s) {

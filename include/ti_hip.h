@@ -410,8 +410,8 @@ int ti_attn_prefill_set_kernel(int mode);
  * place j % page of page table[b * table_ld + j / page]; entries outside [0, pages) are holes: nothing is written there, and no
  * row sees their tokens.  A page belongs to one sequence while it is written.
  *   kv_type TI_KV_SAME: elements of `dtype`;
- *   TI_KV_I8: int8 q, value = q * scale of the token's block of 16 and head, k_scale / v_scale [pages][kv_heads][page / 16], > 0
- *   (NaN: the block's values are none).
+ *   TI_KV_I8: int8 q, value = q * scale of the token's block of 16 and head, k_scale / v_scale [pages][kv_heads][page / 16], 2^-100 ..
+ *   2^121 as ti_paged_append writes them (attention takes a smaller v_scale as 2^-100; NaN: the block's values are none).
  * Rows of a batch are ragged: row i of sequence b (row row_start[b] + i of the call) is its token len[b] - n_b + i, n_b =
  * row_start[b + 1] - row_start[b]; len counts the call's own rows.  row_start (device, [seqs + 1], from 0, not falling) NULL: one
  * row a sequence.  Rows behind the last sequence, and rows whose token lies outside the table (or, rotated, outside the rotation

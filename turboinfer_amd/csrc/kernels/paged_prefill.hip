@@ -12,9 +12,11 @@
 // the registers of two waves a SIMD; they hand each other their weights through LDS, with a reference each (a whole number: moving to the larger is
 // exact).  4000 rows of 16 heads on 8: 308 -> 220 us against one wave with all of it, one a SIMD.
 //
-// Bound: one issue port for matrix products and vector instructions.  4000 rows of 32 heads on 8 of 128: 155 - 160 us (820 - 850 TFLOP/s; 16000 rows 990, a
-// library product 1218), matrix units busy 41 % of the cycles, vector instructions 48 %, LDS 37 %; with a cap 188 - 200 us, 31 % and 61 %; int8 172 - 180.  The waves
-// of a SIMD a part of a step behind each other, by four steps in LDS and barriers at two places: 159 us, 214 with a cap; a barrier every second step 163, 201.
+// Bound: a wave's products and its softmax follow one another, and the other wave of its SIMD fills little of it: no unit is full.  4000 rows of 32 heads on
+// 8 of 128: 148 - 153 us (860 - 890 TFLOP/s; 16000 rows 990, a library product 1218), matrix units busy 41 % of the cycles, vector instructions 48 %, LDS 37 %;
+// with a cap 184 - 189 us, 31 % and 61 %; int8 164; heads of 256 186.  Waves of a SIMD a part of a step behind each other, by four steps in LDS and barriers
+// at two places: 159 us for 159, 214 with a cap for 200; a barrier every second step 163, 201.  Not tried: the next step's scores among this one's softmax in
+// the same wave, which needs both steps' scores in registers.
 #include <math.h>
 
 #include <atomic>

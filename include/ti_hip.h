@@ -415,8 +415,8 @@ int ti_attn_prefill_set_kernel(int mode);
  * Rows of a batch are ragged: row i of sequence b (row row_start[b] + i of the call) is its token len[b] - n_b + i, n_b =
  * row_start[b + 1] - row_start[b]; len counts the call's own rows.  row_start (device, [seqs + 1], from 0, not falling) NULL: one
  * row a sequence.  Rows behind the last sequence, and rows whose token lies outside the table (or, rotated, outside the rotation
- * table), are left as they are (TI_KV_I8: their bytes; the scale of a block that other rows of the call reach is those's); keys past
- * the table are not there.
+ * table), are left as they are (TI_KV_I8: their bytes; a block that other rows of the call reach has the scale that those give it); keys
+ * past the table are not there.
  * head_dim 64, 128 or 256; page 16, 32, 64, 128 or 256; heads a multiple of kv_heads; pages * kv_heads * page / 16 and table_ld *
  * page below 2^31; at most 2^23 rows; k, v and every row 16-byte aligned; all memory on the current device, outputs apart from inputs.  No call reads or writes memory outside the pages of its table, copies to
  * the host or keeps anything for the next; all can be captured into graphs. */

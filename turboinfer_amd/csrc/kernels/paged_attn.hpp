@@ -21,8 +21,8 @@ struct PagedAttn {
   int heads, G, ldq, ldo, window, splits, deal;
   float unit;       // of the denominators: int8 kPagedUnit, else 1
   float f, cap;     // weights are 2^(f s), or with a cap 2^(cap paged_capped(s, f)); caps that are not near: 2^(cap tanh(fx s)) (paged_cap)
-  float fx;
-  int far;          // a cap that is not near
+  float fx;         // scale / the cap, where it is not near
+  int far;          // a cap that is not near (paged_cap_near)
 };
 
 constexpr float kPagedLog2e = 1.44269504088896341f;
@@ -61,7 +61,8 @@ __device__ __forceinline__ uint32_t i8_of(uint32_t x) {
 // A score under a cap c, c tanh(x) = c - 2 c / (e^2x + 1): what 2 c log2 e (PagedAttn::cap) is multiplied with to an exponent of 2, without the
 // first term, which all keys have.  f: 2 scale log2 e / c (int8: times the keys' scale).  Its error goes with the cap, 2^-22 of it.
 __device__ __forceinline__ float paged_capped(float s, float f) { return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s * f)); }
-// So it serves caps of which that is less than a weight's rounding to 16 bits (2^-16 at 64), and with which f stays finite and normal.
+// So it serves caps of which that is less than a weight's rounding to 16 bits (2^-16 at 64), and with which f is a normal number (at 1 / 16 and a scale of
+// 1 also times the keys' largest scale, 2^121).
 static inline bool paged_cap_near(float cap, float scale) { return cap >= 0x1p-4f && cap <= 64.0f && fabsf(scale) >= 0x1p-100f; }
 
 // Any other cap: exponents of 2 in place of the scores, C tanh(x), C = c log2 e (PagedAttn::cap), with errors that go with the score.
